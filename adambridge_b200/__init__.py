@@ -7,11 +7,13 @@ include/abx.h), behind the reference's ``AdamBridge`` / ``OptiComputeAdamW`` /
 the state ZeRO-1 style over the ranks of a process group; the all-gather of the new bf16
 weights is fused into the update as NVLink stores into the peers' copies, or run by NCCL.
 ``clip_coefficient`` computes torch's gradient-clipping norm and coefficient on the device.
+``GraphAdamW`` (``adambridge_b200.graph_adamw``) is AdamW with fp32 or 8-bit moments whose step a CUDA graph can replay.
 """
 
 from . import native, precision
 from .clip import clip_coefficient
 from .engine import StepStats
+from .graph_adamw import GraphAdamW
 from .optimizer import AdamBridge, LionBridge, OptiComputeAdamW
 from .precision import bytes_per_param
 
@@ -19,6 +21,7 @@ __version__ = "0.1.0"
 
 __all__ = [
     "AdamBridge",
+    "GraphAdamW",
     "LionBridge",
     "OptiComputeAdamW",
     "StepStats",

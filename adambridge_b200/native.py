@@ -25,7 +25,7 @@ import torch
 
 from . import _build
 
-__all__ = ["NativeKernels", "Group", "Segment", "State", "StepCoefficients", "load", "build", "available", "mix_seed",
+__all__ = ["NativeKernels", "Group", "Segment", "State", "GraphStep", "StepCoefficients", "load", "build", "available", "mix_seed",
            "SIMD_NAMES", "BuildError", "LIBRARY"]
 
 log = logging.getLogger("adambridge_b200.native")
@@ -35,6 +35,9 @@ LIBRARY = _build.LIB
 SIMD_NAMES = {0: "scalar", 1: "avx2", 2: "avx512", 3: "neon"}
 
 DT_NONE, DT_F32, DT_BF16, DT_FP8, DT_F24 = 0, 1, 2, 3, 4
+DT_I8 = 5                 # 8-bit moments of graph_adamw
+I8_BLOCK = 256            # values per scale of an 8-bit moment
+GRAPH_TENSOR_WORDS = 10   # 8-byte words of one abx_graph_tensor
 _DTYPE_CODES = {torch.float32: DT_F32, torch.bfloat16: DT_BF16}
 MOMENT_CODES = {"fp32": DT_F32, "bf16": DT_BF16, "fp8": DT_FP8}
 MASTER_CODES = {"fp32": DT_F32, "fp24": DT_F24}
@@ -123,6 +126,26 @@ class Segment(ctypes.Structure):
         ("algorithm", ctypes.c_int32),  # ALGORITHMS; Lion leaves v, v_scale NULL
         ("p_dtype", ctypes.c_int32),    # MASTER_CODES (0 means fp32)
         ("reserved", ctypes.c_int32),
+    ]
+
+
+class GraphStep(ctypes.Structure):
+    """What the tensors of one graph_adamw call share (abx_graph_step)."""
+
+    _fields_ = [
+        ("lr", ctypes.c_double),
+        ("beta1", ctypes.c_double),
+        ("beta2", ctypes.c_double),
+        ("eps", ctypes.c_double),
+        ("weight_decay", ctypes.c_double),
+        ("lr_ptr", ctypes.c_void_p),
+        ("g_scale", ctypes.c_void_p),
+        ("skip", ctypes.c_void_p),
+        ("norm", ctypes.c_void_p),
+        ("lr_f64", ctypes.c_int32),
+        ("moments", ctypes.c_int32),
+        ("stochastic", ctypes.c_int32),
+        ("seed", ctypes.c_uint32),
     ]
 
 
@@ -247,6 +270,17 @@ class NativeKernels:
         lib.abx_clip_coef_noalloc.restype = ctypes.c_int
         lib.abx_clip_coef_noalloc.argtypes = [ctypes.c_void_p, tens, ctypes.c_int32, ctypes.c_float, ctypes.c_void_p,
                                               ctypes.c_void_p, ctypes.c_void_p]
+        for fn, size in (("abx_graph_tensor_size", 8 * GRAPH_TENSOR_WORDS), ("abx_graph_step_size", ctypes.sizeof(GraphStep))):
+            getattr(lib, fn).restype = ctypes.c_int
+            if getattr(lib, fn)() != size:
+                raise BuildError(f"{fn}: struct layout mismatch between C and Python")
+        lib.abx_graph_adamw.restype = ctypes.c_int
+        lib.abx_graph_adamw.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.POINTER(GraphStep),
+                                        ctypes.c_void_p, ctypes.c_int32]
+        for fn in ("abx_i8_decode", "abx_i8_encode"):
+            getattr(lib, fn).restype = ctypes.c_int
+            getattr(lib, fn).argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                                         ctypes.c_int64, ctypes.c_int32]
         self._lib = lib
 
     # -- rounding pattern ----------------------------------------------------
@@ -414,6 +448,44 @@ class NativeKernels:
         """Enqueue the conversion of n values from state buffer ``src`` to ``dst`` (abx_convert) on ``stream``."""
         rc = self._lib.abx_convert(_stream_handle(stream), ctypes.byref(src), ctypes.byref(dst), int(n))
         self._check(rc, "abx_convert")
+
+    # -- AdamW whose step lives on the device ----------------------------------
+
+    def graph_adamw(self, stream, tensors: torch.Tensor, shared: GraphStep, ticket: torch.Tensor, max_ctas: int = 0) -> None:
+        """Enqueue abx_graph_adamw on ``stream``: ``tensors`` is a host int64 table, one abx_graph_tensor per row;
+        ``ticket`` a one-element int32 CUDA tensor, zero before the first call."""
+        if tensors.dtype != torch.int64 or tensors.is_cuda or not tensors.is_contiguous() or (
+                tensors.dim() != 2 or tensors.shape[1] != GRAPH_TENSOR_WORDS):
+            raise ValueError(f"tensors must be a contiguous host int64 table of {GRAPH_TENSOR_WORDS} words per row")
+        if not ticket.is_cuda or ticket.dtype != torch.int32 or ticket.numel() != 1:
+            raise ValueError("ticket must be a one-element int32 CUDA tensor")
+        rc = self._lib.abx_graph_adamw(_stream_handle(stream), tensors.data_ptr(), len(tensors), ctypes.byref(shared),
+                                       ticket.data_ptr(), max_ctas)
+        self._check(rc, "abx_graph_adamw")
+
+    def i8_decode(self, stream, codes: torch.Tensor, scales: torch.Tensor, values: torch.Tensor, role: str) -> None:
+        """values = the fp32 values of 8-bit moments (``role`` 'm' or 'v')."""
+        self._i8(codes, scales, values)
+        rc = self._lib.abx_i8_decode(_stream_handle(stream), codes.data_ptr(), scales.data_ptr(), values.data_ptr(),
+                                     values.numel(), int(role == "v"))
+        self._check(rc, "abx_i8_decode")
+
+    def i8_encode(self, stream, values: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, role: str) -> None:
+        """codes, scales = the nearest 8-bit moments of fp32 values (``role`` 'm' or 'v')."""
+        self._i8(codes, scales, values)
+        rc = self._lib.abx_i8_encode(_stream_handle(stream), values.data_ptr(), codes.data_ptr(), scales.data_ptr(),
+                                     values.numel(), int(role == "v"))
+        self._check(rc, "abx_i8_encode")
+
+    @staticmethod
+    def _i8(codes: torch.Tensor, scales: torch.Tensor, values: torch.Tensor) -> None:
+        blocks = -(-values.numel() // I8_BLOCK)
+        if not all(t.is_cuda and t.is_contiguous() and t.device == values.device for t in (codes, scales, values)):
+            raise ValueError("codes, scales and values must be contiguous CUDA tensors of one device")
+        if codes.element_size() != 1 or scales.dtype != torch.float32 or values.dtype != torch.float32:
+            raise TypeError("8-bit codes, float32 scales and float32 values are needed")
+        if codes.numel() < blocks * I8_BLOCK or scales.numel() < blocks:
+            raise ValueError(f"{values.numel()} values need {blocks} whole blocks of codes and as many scales")
 
     @staticmethod
     def make_hparams(c: StepCoefficients, seed: int, stochastic: bool) -> _HParams:

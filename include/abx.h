@@ -40,7 +40,9 @@ enum {
     ABX_DT_F32  = 1,
     ABX_DT_BF16 = 2,
     ABX_DT_FP8  = 3,  /* moments: E4M3fn m, E5M2 sqrt(v), one fp32 scale per 128 elements */
-    ABX_DT_F24  = 4   /* master: bf16 hi plane + uint8 lo plane (top 24 bits of fp32) */
+    ABX_DT_F24  = 4,  /* master: bf16 hi plane + uint8 lo plane (top 24 bits of fp32) */
+    ABX_DT_I8   = 5   /* moments of abx_graph_adamw: int8 codes of m, uint8 codes of sqrt(v), one fp32 scale
+                         per ABX_I8_BLOCK values */
 };
 
 /* Update rules; same codes as the reference (adambridge_kernels.c:75). */
@@ -52,6 +54,7 @@ enum { ABX_ALGO_ADAMW = 0, ABX_ALGO_LION = 1 };
 enum { ABX_SIMD_SCALAR = 0, ABX_SIMD_AVX2 = 1, ABX_SIMD_AVX512 = 2, ABX_SIMD_NEON = 3 };
 
 #define ABX_FP8_BLOCK 128
+#define ABX_I8_BLOCK 256
 
 /* Error codes.  -1 .. -13 have the reference's meaning (check_segment,
  * adambridge_kernels.c:1537-1553, and adambridge_multi_step :1611-1626). */
@@ -272,6 +275,63 @@ typedef struct abx_state {
  * ABX_E_MV_DTYPE, ABX_E_NULL_PTR, ABX_E_SCALE_NULL (FP8 scales or the fp24 lo plane
  * missing), ABX_E_ALIGN; ABX_E_CUDA on a launch failure. */
 int abx_convert(void* stream, const abx_state* src, const abx_state* dst, int64_t n);
+
+/* ---- AdamW whose step lives on the device ------------------------------------------------
+ * No counterpart in the reference.  Step counts, and where wanted the learning rate, the
+ * gradient scale and the decision to skip the step, are device memory, so a CUDA graph that
+ * captured the call performs the next step at every replay. */
+
+/* One tensor.  m, v, the scales and master are padded to whole ABX_I8_BLOCK blocks (the
+ * padding stays zero) and start on 16-byte boundaries (the scales on 4-byte ones). */
+typedef struct abx_graph_tensor {
+    void* w;            /* the weights, dtype; fp32 weights are their own master */
+    const void* g;      /* the gradient, dtype */
+    float* master;      /* fp32 master of bf16 weights; unused for fp32 weights */
+    void* m;            /* first moment: float[], or int8 codes */
+    void* v;            /* second moment: float[], or uint8 codes of its square root */
+    float* m_scale;     /* ABX_DT_I8 only: one scale per block */
+    float* v_scale;
+    int64_t* step;      /* device: steps taken; incremented unless the step is skipped */
+    int64_t n;
+    uint32_t index;     /* selects the rounding stream; below 2^31 */
+    int32_t dtype;      /* of w and g: ABX_DT_F32 or ABX_DT_BF16 */
+} abx_graph_tensor;
+
+/* What the tensors of a call share.  Pointers are device pointers, or NULL. */
+typedef struct abx_graph_step {
+    double lr;
+    double beta1;
+    double beta2;
+    double eps;
+    double weight_decay;
+    const void* lr_ptr;     /* replaces lr: one double (lr_f64 != 0) or float */
+    const float* g_scale;   /* multiplies every gradient value, in fp32 */
+    const float* skip;      /* nonzero (or NaN): nothing changes */
+    const float* norm;      /* not finite: nothing changes */
+    int32_t lr_f64;
+    int32_t moments;        /* ABX_DT_F32 or ABX_DT_I8 */
+    int32_t stochastic;     /* ABX_DT_I8: round the codes at random (unbiased) instead of to the nearest */
+    uint32_t seed;
+} abx_graph_step;
+
+int abx_graph_tensor_size(void);
+int abx_graph_step_size(void);
+
+/* Enqueue one AdamW step of n tensors on `stream` (a tensor occurs once; an empty one is left
+ * out and its step count kept).  ticket: one word of device memory, 0 before the first call;
+ * every call leaves it 0, and calls that may overlap on the device need their own.  max_ctas
+ * caps the CTAs of a launch (0: all resident).  One launch per 384 tensors of a dtype.
+ * Everything is checked before anything is launched.  Errors: ABX_E_ARG, ABX_E_G_DTYPE,
+ * ABX_E_MV_DTYPE, ABX_E_NULL_PTR, ABX_E_SCALE_NULL, ABX_E_ALIGN, ABX_E_CUDA. */
+int abx_graph_adamw(void* stream, const abx_graph_tensor* tensors, int32_t n, const abx_graph_step* step,
+                    uint32_t* ticket, int32_t max_ctas);
+
+/* Moments between ABX_DT_I8 and fp32, n values; role 0: m = code * scale, 1: v = (code * scale)^2.
+ * Encoding takes the nearest code (at least 1 for v > 0; a negative v counts as 0) and writes whole
+ * blocks.  codes start on an 8-byte boundary.  Errors: ABX_E_ARG, ABX_E_NULL_PTR, ABX_E_SCALE_NULL,
+ * ABX_E_ALIGN, ABX_E_CUDA. */
+int abx_i8_decode(void* stream, const void* codes, const float* scales, float* values, int64_t n, int32_t role);
+int abx_i8_encode(void* stream, const float* values, void* codes, float* scales, int64_t n, int32_t role);
 
 /* Kernel launches this library has made in this process, all threads and devices. */
 uint64_t abx_launch_count(void);
