@@ -8,12 +8,14 @@ the state ZeRO-1 style over the ranks of a process group; the all-gather of the 
 weights is fused into the update as NVLink stores into the peers' copies, or run by NCCL.
 ``clip_coefficient`` computes torch's gradient-clipping norm and coefficient on the device.
 ``GraphAdamW`` (``adambridge_b200.graph_adamw``) is AdamW with fp32 or 8-bit moments whose step a CUDA graph can replay.
+``layer_norm`` and ``rms_norm`` (``adambridge_b200.norm``) are the norms of a training step, with their backward passes.
 """
 
 from . import native, precision
 from .clip import clip_coefficient
 from .engine import StepStats
 from .graph_adamw import GraphAdamW
+from .norm import layer_norm, rms_norm
 from .optimizer import AdamBridge, LionBridge, OptiComputeAdamW
 from .precision import bytes_per_param
 
@@ -27,7 +29,9 @@ __all__ = [
     "StepStats",
     "bytes_per_param",
     "clip_coefficient",
+    "layer_norm",
     "native",
     "precision",
+    "rms_norm",
     "__version__",
 ]

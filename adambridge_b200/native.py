@@ -25,7 +25,7 @@ import torch
 
 from . import _build
 
-__all__ = ["NativeKernels", "Group", "Segment", "State", "GraphStep", "StepCoefficients", "load", "build", "available", "mix_seed",
+__all__ = ["NativeKernels", "Group", "Segment", "State", "GraphStep", "Norm", "StepCoefficients", "load", "build", "available", "mix_seed",
            "SIMD_NAMES", "BuildError", "LIBRARY"]
 
 log = logging.getLogger("adambridge_b200.native")
@@ -146,6 +146,23 @@ class GraphStep(ctypes.Structure):
         ("moments", ctypes.c_int32),
         ("stochastic", ctypes.c_int32),
         ("seed", ctypes.c_uint32),
+    ]
+
+
+class Norm(ctypes.Structure):
+    """One layer norm or RMS norm over rows (abx_norm)."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("w", ctypes.c_void_p),
+        ("b", ctypes.c_void_p),
+        ("rows", ctypes.c_int64),
+        ("cols", ctypes.c_int64),
+        ("x_stride", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("w_dtype", ctypes.c_int32),
+        ("rms", ctypes.c_int32),
+        ("eps", ctypes.c_float),
     ]
 
 
@@ -270,7 +287,8 @@ class NativeKernels:
         lib.abx_clip_coef_noalloc.restype = ctypes.c_int
         lib.abx_clip_coef_noalloc.argtypes = [ctypes.c_void_p, tens, ctypes.c_int32, ctypes.c_float, ctypes.c_void_p,
                                               ctypes.c_void_p, ctypes.c_void_p]
-        for fn, size in (("abx_graph_tensor_size", 8 * GRAPH_TENSOR_WORDS), ("abx_graph_step_size", ctypes.sizeof(GraphStep))):
+        for fn, size in (("abx_graph_tensor_size", 8 * GRAPH_TENSOR_WORDS), ("abx_graph_step_size", ctypes.sizeof(GraphStep)),
+                         ("abx_norm_size", ctypes.sizeof(Norm))):
             getattr(lib, fn).restype = ctypes.c_int
             if getattr(lib, fn)() != size:
                 raise BuildError(f"{fn}: struct layout mismatch between C and Python")
@@ -281,6 +299,14 @@ class NativeKernels:
             getattr(lib, fn).restype = ctypes.c_int
             getattr(lib, fn).argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                          ctypes.c_int64, ctypes.c_int32]
+        norm = ctypes.POINTER(Norm)
+        lib.abx_norm_forward.restype = ctypes.c_int
+        lib.abx_norm_forward.argtypes = [ctypes.c_void_p, norm, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
+        lib.abx_norm_backward_workspace_bytes.restype = ctypes.c_size_t
+        lib.abx_norm_backward_workspace_bytes.argtypes = [norm]
+        lib.abx_norm_backward.restype = ctypes.c_int
+        lib.abx_norm_backward.argtypes = [ctypes.c_void_p, norm, ctypes.c_void_p, ctypes.c_int64, *[ctypes.c_void_p] * 6,
+                                          ctypes.c_size_t]
         self._lib = lib
 
     # -- rounding pattern ----------------------------------------------------
@@ -476,6 +502,30 @@ class NativeKernels:
         rc = self._lib.abx_i8_encode(_stream_handle(stream), values.data_ptr(), codes.data_ptr(), scales.data_ptr(),
                                      values.numel(), int(role == "v"))
         self._check(rc, "abx_i8_encode")
+
+    # -- layer norm and RMS norm --------------------------------------------------
+
+    def norm_forward(self, stream, norm: Norm, y: torch.Tensor, stats: torch.Tensor | None) -> None:
+        """y = the norm of the rows that ``norm`` describes; ``stats`` (fp32, [2 or 1 for RMS, rows]) receives rstd and
+        the mean."""
+        rstd = None if stats is None else stats.data_ptr()
+        mean = None if stats is None or norm.rms else rstd + 4 * norm.rows
+        rc = self._lib.abx_norm_forward(_stream_handle(stream), ctypes.byref(norm), y.data_ptr(), mean, rstd)
+        self._check(rc, "abx_norm_forward")
+
+    def norm_backward(self, stream, norm: Norm, dy: torch.Tensor, dy_stride: int, stats: torch.Tensor,
+                      dx: torch.Tensor | None, dw: torch.Tensor | None, db: torch.Tensor | None) -> None:
+        """The gradients that are not None, from ``dy`` and the forward pass's statistics."""
+        rstd = stats.data_ptr()
+        mean = None if norm.rms else rstd + 4 * norm.rows
+        ref, ws, size = ctypes.byref(norm), None, 0
+        if dw is not None or db is not None:
+            size = self._lib.abx_norm_backward_workspace_bytes(ref)
+            ws = torch.empty(size, dtype=torch.uint8, device=stats.device)
+        ptr = lambda t: None if t is None else t.data_ptr()   # noqa: E731
+        rc = self._lib.abx_norm_backward(_stream_handle(stream), ref, dy.data_ptr(), dy_stride, mean, rstd, ptr(dx), ptr(dw),
+                                         ptr(db), ptr(ws), size)
+        self._check(rc, "abx_norm_backward")
 
     @staticmethod
     def _i8(codes: torch.Tensor, scales: torch.Tensor, values: torch.Tensor) -> None:

@@ -333,6 +333,37 @@ int abx_graph_adamw(void* stream, const abx_graph_tensor* tensors, int32_t n, co
 int abx_i8_decode(void* stream, const void* codes, const float* scales, float* values, int64_t n, int32_t role);
 int abx_i8_encode(void* stream, const float* values, void* codes, float* scales, int64_t n, int32_t role);
 
+/* ---- layer norm and RMS norm over the last axis -------------------------------------------
+ * No counterpart in the reference.  Rows of cols values; statistics and sums in fp32. */
+typedef struct abx_norm {
+    const void* x;       /* rows, dtype; x_stride elements from one to the next */
+    const void* w;       /* cols weights, w_dtype; NULL: 1 */
+    const void* b;       /* cols biases, w_dtype; NULL: 0 (and always for RMS norm) */
+    int64_t rows;
+    int64_t cols;        /* at least 1 */
+    int64_t x_stride;
+    int32_t dtype;       /* of x, y, dy, dx: ABX_DT_F32 or ABX_DT_BF16 */
+    int32_t w_dtype;     /* of w, b, dw, db: ABX_DT_F32 or ABX_DT_BF16 */
+    int32_t rms;         /* nonzero: RMS norm (no mean, no bias) */
+    float eps;
+} abx_norm;
+
+int abx_norm_size(void);
+
+/* y (contiguous rows) = (x - mean) rstd w + b.  mean and rstd receive the rows' statistics, for the
+ * backward pass; NULL where they are not wanted.  Errors: ABX_E_ARG, ABX_E_G_DTYPE (dtype),
+ * ABX_E_P_DTYPE (w_dtype), ABX_E_NULL_PTR, ABX_E_ALIGN, ABX_E_CUDA. */
+int abx_norm_forward(void* stream, const abx_norm* norm, void* y, float* mean, float* rstd);
+
+/* The gradients from dy (dy_stride elements from row to row) and the forward pass's statistics: dx
+ * (contiguous rows), dw and db (cols values), each NULL where not wanted.  dw and db are sums over the
+ * rows in fp32 in an order fixed by the sizes and the device, rounded once; they need a workspace of
+ * abx_norm_backward_workspace_bytes (for the current device; 16-byte aligned), written and read by this
+ * call alone.  Errors: those of abx_norm_forward, and ABX_E_OOM for a workspace that is too small. */
+size_t abx_norm_backward_workspace_bytes(const abx_norm* norm);
+int abx_norm_backward(void* stream, const abx_norm* norm, const void* dy, int64_t dy_stride, const float* mean,
+                      const float* rstd, void* dx, void* dw, void* db, void* workspace, size_t workspace_bytes);
+
 /* Kernel launches this library has made in this process, all threads and devices. */
 uint64_t abx_launch_count(void);
 
