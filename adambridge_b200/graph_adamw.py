@@ -22,7 +22,7 @@ master; fp32 parameters are updated in place.
 
 from __future__ import annotations
 
-from operator import attrgetter
+import ctypes
 from typing import Any, Callable, Iterable
 
 import torch
@@ -36,10 +36,6 @@ __all__ = ["GraphAdamW", "StateArena"]
 BLOCK = native.I8_BLOCK
 _PRECISIONS = ("fp32", "int8")
 _CODES = {"m": torch.int8, "v": torch.uint8}
-_WORDS = native.GRAPH_TENSOR_WORDS
-_grad, _dtype = attrgetter("grad"), attrgetter("dtype")
-_numel, _data_ptr = torch.Tensor.numel, torch.Tensor.data_ptr
-_is_contiguous, _get_device = torch.Tensor.is_contiguous, torch.Tensor.get_device
 
 
 def _padded(n: int) -> int:
@@ -54,7 +50,7 @@ class StateArena:
     parameter; the buffer is None if the group has no bf16 one); ``steps``: steps taken, int64 per parameter.
     Values between a parameter's end and the next boundary are zero and stay zero."""
 
-    def __init__(self, params: list[torch.Tensor], first_index: int, precision: str, kernels: native.NativeKernels):
+    def __init__(self, params: list[torch.Tensor], first_index: int, precision: str):
         for p in params:
             if not p.is_cuda:
                 raise ValueError("adambridge_b200 updates CUDA parameters only (the state lives in GPU memory)")
@@ -64,7 +60,7 @@ class StateArena:
                 raise ValueError("non-contiguous parameters are not supported")
             if p.dtype not in (torch.float32, torch.bfloat16):
                 raise TypeError(f"parameters must be float32 or bfloat16, got {p.dtype}")
-        self.params, self.precision, self.first_index, self._native = params, precision, first_index, kernels
+        self.params, self.precision, self.first_index, self._ops = params, precision, first_index, native.torch_ops()
         dev = self.device = params[0].device
         self.numels, self.dtypes = [p.numel() for p in params], [p.dtype for p in params]
         self.offsets: list[int] = []
@@ -102,44 +98,14 @@ class StateArena:
                          (first_index + i) | (native.dtype_code_of(dt) << 32)])
         self._table = torch.tensor(rows, dtype=torch.int64)
 
-    def describe(self, grads: list[torch.Tensor | None]) -> tuple[torch.Tensor, list]:
-        """The kernel descriptions of the parameters that have a gradient, as a host table, and the tensors that must
-        live until the launch.  Parameters and gradients are checked and their addresses taken now."""
-        params, numels, dtypes, table = self.params, self.numels, self.dtypes, self._table
-        if any(g is None for g in grads):
-            have = [i for i, g in enumerate(grads) if g is not None]
-            params, grads = [params[i] for i in have], [grads[i] for i in have]
-            numels, dtypes = [numels[i] for i in have], [dtypes[i] for i in have]
-            table = table[have]
-        else:
-            table = table.clone()
-        if not grads:
-            return table, []
-        for what in (params, grads):
-            if (list(map(_dtype, what)) != dtypes or list(map(_numel, what)) != numels
-                    or set(map(_get_device, what)) != {self.device.index}):
-                self._refuse(params, grads, dtypes, numels)
-        if not all(map(_is_contiguous, params)):
-            raise ValueError("non-contiguous parameters are not supported")
-        if any(g.is_sparse for g in grads):
-            raise RuntimeError("GraphAdamW does not support sparse gradients")
-        if not all(map(_is_contiguous, grads)):
-            grads = [g.contiguous() for g in grads]
-        table[:, 0] = torch.tensor(list(map(_data_ptr, params)), dtype=torch.int64)
-        table[:, 1] = torch.tensor(list(map(_data_ptr, grads)), dtype=torch.int64)
-        return table, grads
+    def describe(self):
+        """The kernel's descriptions of the parameters that have a gradient: parameters and gradients are checked and
+        their addresses taken now."""
+        return self._ops.describe_step(self.params, self._table, self.device.index)
 
-    def _refuse(self, params, grads, dtypes, numels) -> None:
-        for p, g, dt, n in zip(params, grads, dtypes, numels):
-            if p.dtype != dt or p.numel() != n or p.device != self.device:
-                raise RuntimeError(f"a parameter changed after its state was made ({n} x {dt} on {self.device}, now "
-                                   f"{p.numel()} x {p.dtype} on {p.device})")
-            if g.is_sparse:
-                raise RuntimeError("GraphAdamW does not support sparse gradients")
-            if g.dtype != dt:
-                raise TypeError(f"the gradient of a {dt} parameter must be {dt}, got {g.dtype}")
-            if g.numel() != n or g.device != self.device:
-                raise ValueError(f"a gradient has {g.numel()} elements on {g.device}, its parameter {n} on {self.device}")
+    def launch(self, described, shared: native.GraphStep, max_ctas: int) -> None:
+        """Enqueue the step of what :meth:`describe` returned, on the current stream."""
+        self._ops.launch_step(described, ctypes.addressof(shared), self.ticket, max_ctas)
 
     # ------------------------------------------------------------------ reading and writing the moments
 
@@ -150,10 +116,7 @@ class StateArena:
         plane, scales = self._plane(role)
         if scales is None:
             return plane
-        out = torch.empty(self.numel, dtype=torch.float32, device=self.device)
-        with torch.cuda.device(self.device):
-            self._native.i8_decode(None, plane, scales, out, role)
-        return out
+        return self._ops.i8_decode(plane, scales, self.numel, role == "v")
 
     def exp_avg(self) -> torch.Tensor:
         """The first moments as flat fp32 (``numel`` values, parameter ``i`` from ``offsets[i]``): the live buffer, or
@@ -179,10 +142,7 @@ class StateArena:
         codes, scale = plane[at:end], scales[at // BLOCK:end // BLOCK]
         if not as_fp32:
             return {"precision": "int8", "role": role, "block": BLOCK, "q": codes, "scale": scale}
-        out = torch.empty(n, dtype=torch.float32, device=self.device)
-        with torch.cuda.device(self.device):
-            self._native.i8_decode(None, codes, scale, out, role)
-        return {"precision": "fp32", "data": out}
+        return {"precision": "fp32", "data": self._ops.i8_decode(codes, scale, n, role == "v")}
 
     def load_moment(self, i: int, role: str, saved: "dict | StateBuffer") -> None:
         """Write a checked checkpoint moment: int8 planes as they are, other formats by their values."""
@@ -193,17 +153,15 @@ class StateArena:
             plane[at:end].copy_(saved["q"].reshape(-1))
             scales[at // BLOCK:end // BLOCK].copy_(saved["scale"].reshape(-1))
             return
-        with torch.cuda.device(self.device):
-            if isinstance(saved, dict):
-                values = torch.empty(n, dtype=torch.float32, device=self.device)
-                self._native.i8_decode(None, saved["q"].reshape(-1).to(self.device).contiguous(),
-                                       saved["scale"].reshape(-1).to(self.device).contiguous(), values, role)
-            else:
-                values = saved.to_device(self.device).to_fp32()
-            if scales is None:
-                plane[at:at + n].copy_(values)
-            elif n:
-                self._native.i8_encode(None, values, plane[at:end], scales[at // BLOCK:end // BLOCK], role)
+        if isinstance(saved, dict):
+            q, scale = (saved[name].reshape(-1).to(self.device).contiguous() for name in ("q", "scale"))
+            values = self._ops.i8_decode(q, scale, n, role == "v")
+        else:
+            values = saved.to_device(self.device).to_fp32()
+        if scales is None:
+            plane[at:at + n].copy_(values)
+        else:
+            self._ops.i8_encode(values, plane[at:end], scales[at // BLOCK:end // BLOCK], role == "v")
 
     @property
     def nbytes(self) -> dict[str, int]:
@@ -291,7 +249,7 @@ class GraphAdamW(torch.optim.Optimizer):
                 raise RuntimeError("GraphAdamW: make the state before a capture (prepare(), or an uncaptured step)")
             first = sum(len(a.params) for a in self.arenas)
             for group in self.param_groups[len(self.arenas):]:
-                self.arenas.append(StateArena(group["params"], first, self.precision, self._native))
+                self.arenas.append(StateArena(group["params"], first, self.precision))
                 first += len(group["params"])
         return self
 
@@ -314,13 +272,10 @@ class GraphAdamW(torch.optim.Optimizer):
         coef, norm = clip if clip is not None else (grad_scale, None)
         self.prepare()
         # every group is described, and so checked, before any is launched
-        work = [(arena, group, *arena.describe(list(map(_grad, arena.params))))
+        work = [(arena, arena.describe(), self._shared(arena, group, coef, found_inf, norm))
                 for arena, group in zip(self.arenas, self.param_groups)]
-        work = [(arena, self._shared(arena, group, coef, found_inf, norm), table, keep)
-                for arena, group, table, keep in work if len(table)]
-        for arena, shared, table, keep in work:
-            with torch.cuda.device(arena.device):
-                self._native.graph_adamw(None, table, shared, arena.ticket, self.max_ctas)
+        for arena, described, shared in work:
+            arena.launch(described, shared, self.max_ctas)
         return loss
 
     def _shared(self, arena: StateArena, group: dict[str, Any], coef, found_inf, norm) -> native.GraphStep:

@@ -16,6 +16,7 @@ load, ``load()`` raises.  Build it with ``python -m adambridge_b200._build``.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import logging
 import threading
 from dataclasses import dataclass
@@ -25,7 +26,7 @@ import torch
 
 from . import _build
 
-__all__ = ["NativeKernels", "Group", "Segment", "State", "GraphStep", "Norm", "StepCoefficients", "load", "build", "available", "mix_seed",
+__all__ = ["NativeKernels", "Group", "Segment", "State", "GraphStep", "Norm", "StepCoefficients", "load", "build", "available", "mix_seed", "torch_ops",
            "SIMD_NAMES", "BuildError", "LIBRARY"]
 
 log = logging.getLogger("adambridge_b200.native")
@@ -475,68 +476,6 @@ class NativeKernels:
         rc = self._lib.abx_convert(_stream_handle(stream), ctypes.byref(src), ctypes.byref(dst), int(n))
         self._check(rc, "abx_convert")
 
-    # -- AdamW whose step lives on the device ----------------------------------
-
-    def graph_adamw(self, stream, tensors: torch.Tensor, shared: GraphStep, ticket: torch.Tensor, max_ctas: int = 0) -> None:
-        """Enqueue abx_graph_adamw on ``stream``: ``tensors`` is a host int64 table, one abx_graph_tensor per row;
-        ``ticket`` a one-element int32 CUDA tensor, zero before the first call."""
-        if tensors.dtype != torch.int64 or tensors.is_cuda or not tensors.is_contiguous() or (
-                tensors.dim() != 2 or tensors.shape[1] != GRAPH_TENSOR_WORDS):
-            raise ValueError(f"tensors must be a contiguous host int64 table of {GRAPH_TENSOR_WORDS} words per row")
-        if not ticket.is_cuda or ticket.dtype != torch.int32 or ticket.numel() != 1:
-            raise ValueError("ticket must be a one-element int32 CUDA tensor")
-        rc = self._lib.abx_graph_adamw(_stream_handle(stream), tensors.data_ptr(), len(tensors), ctypes.byref(shared),
-                                       ticket.data_ptr(), max_ctas)
-        self._check(rc, "abx_graph_adamw")
-
-    def i8_decode(self, stream, codes: torch.Tensor, scales: torch.Tensor, values: torch.Tensor, role: str) -> None:
-        """values = the fp32 values of 8-bit moments (``role`` 'm' or 'v')."""
-        self._i8(codes, scales, values)
-        rc = self._lib.abx_i8_decode(_stream_handle(stream), codes.data_ptr(), scales.data_ptr(), values.data_ptr(),
-                                     values.numel(), int(role == "v"))
-        self._check(rc, "abx_i8_decode")
-
-    def i8_encode(self, stream, values: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, role: str) -> None:
-        """codes, scales = the nearest 8-bit moments of fp32 values (``role`` 'm' or 'v')."""
-        self._i8(codes, scales, values)
-        rc = self._lib.abx_i8_encode(_stream_handle(stream), values.data_ptr(), codes.data_ptr(), scales.data_ptr(),
-                                     values.numel(), int(role == "v"))
-        self._check(rc, "abx_i8_encode")
-
-    # -- layer norm and RMS norm --------------------------------------------------
-
-    def norm_forward(self, stream, norm: Norm, y: torch.Tensor, stats: torch.Tensor | None) -> None:
-        """y = the norm of the rows that ``norm`` describes; ``stats`` (fp32, [2 or 1 for RMS, rows]) receives rstd and
-        the mean."""
-        rstd = None if stats is None else stats.data_ptr()
-        mean = None if stats is None or norm.rms else rstd + 4 * norm.rows
-        rc = self._lib.abx_norm_forward(_stream_handle(stream), ctypes.byref(norm), y.data_ptr(), mean, rstd)
-        self._check(rc, "abx_norm_forward")
-
-    def norm_backward(self, stream, norm: Norm, dy: torch.Tensor, dy_stride: int, stats: torch.Tensor,
-                      dx: torch.Tensor | None, dw: torch.Tensor | None, db: torch.Tensor | None) -> None:
-        """The gradients that are not None, from ``dy`` and the forward pass's statistics."""
-        rstd = stats.data_ptr()
-        mean = None if norm.rms else rstd + 4 * norm.rows
-        ref, ws, size = ctypes.byref(norm), None, 0
-        if dw is not None or db is not None:
-            size = self._lib.abx_norm_backward_workspace_bytes(ref)
-            ws = torch.empty(size, dtype=torch.uint8, device=stats.device)
-        ptr = lambda t: None if t is None else t.data_ptr()   # noqa: E731
-        rc = self._lib.abx_norm_backward(_stream_handle(stream), ref, dy.data_ptr(), dy_stride, mean, rstd, ptr(dx), ptr(dw),
-                                         ptr(db), ptr(ws), size)
-        self._check(rc, "abx_norm_backward")
-
-    @staticmethod
-    def _i8(codes: torch.Tensor, scales: torch.Tensor, values: torch.Tensor) -> None:
-        blocks = -(-values.numel() // I8_BLOCK)
-        if not all(t.is_cuda and t.is_contiguous() and t.device == values.device for t in (codes, scales, values)):
-            raise ValueError("codes, scales and values must be contiguous CUDA tensors of one device")
-        if codes.element_size() != 1 or scales.dtype != torch.float32 or values.dtype != torch.float32:
-            raise TypeError("8-bit codes, float32 scales and float32 values are needed")
-        if codes.numel() < blocks * I8_BLOCK or scales.numel() < blocks:
-            raise ValueError(f"{values.numel()} values need {blocks} whole blocks of codes and as many scales")
-
     @staticmethod
     def make_hparams(c: StepCoefficients, seed: int, stochastic: bool) -> _HParams:
         return _HParams(c.beta1, c.beta2, 1.0 - c.beta1, 1.0 - c.beta2, c.decay, c.step_size, c.inv_sqrt_bc2, c.eps,
@@ -581,11 +520,14 @@ def _scale_ptr(g_scale: torch.Tensor) -> int:
 
 _lock = threading.Lock()
 _loaded: NativeKernels | None = None
+_torch_ops = None
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile libabx in-tree (nvcc, sm_100a)."""
-    return _build.build(force=force, verbose=verbose)
+    """Compile libabx (nvcc, sm_100a) and the torch module in-tree; returns libabx's path."""
+    path = _build.build(force=force, verbose=verbose)
+    _build.build_torch(force=force, verbose=verbose)
+    return path
 
 
 def load() -> NativeKernels:
@@ -597,6 +539,27 @@ def load() -> NativeKernels:
                 raise BuildError(f"{LIBRARY} is missing; build it with `python -m adambridge_b200._build`")
             _loaded = NativeKernels(LIBRARY)
         return _loaded
+
+
+def torch_ops():
+    """The module that calls libabx's norms and device-resident step on torch tensors (csrc/abx_torch.cpp), which links
+    libabx.  Raises if it is missing or does not load."""
+    global _torch_ops
+    if _torch_ops is None:
+        load()
+        with _lock:
+            if _torch_ops is None:
+                path = _build.TORCH_LIB
+                if not path.exists():
+                    raise BuildError(f"{path} is missing; build it with `python -m adambridge_b200._build`")
+                spec = importlib.util.spec_from_file_location("_abx_torch", path)
+                try:
+                    module = importlib.util.module_from_spec(spec)
+                    spec.loader.exec_module(module)
+                except ImportError as exc:
+                    raise BuildError(f"cannot load {path}: {exc}") from exc
+                _torch_ops = module
+    return _torch_ops
 
 
 def available() -> bool:
