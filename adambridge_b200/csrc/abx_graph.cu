@@ -42,7 +42,7 @@ using abx::f2u;
 using abx::u2f;
 
 constexpr int kBlock = ABX_I8_BLOCK;      // values per scale: 8 per lane of a warp
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTile = kWarps * kBlock;    // elements of one tensor that a CTA takes at a time
 constexpr int kMany = 384;                // tensors per launch: the parameter block stays under 32764 bytes
@@ -63,7 +63,7 @@ struct Item {
     int64_t* step;
     int64_t n;
     int32_t tile_begin;   // first tile in the launch's tile space
-    uint32_t index_vec;   // index << 1 | (w and g start on 16-byte boundaries)
+    uint32_t index_vec;   // index << 1 | (8 values of w and g can be accessed at once)
 };
 
 template <int N>
@@ -79,6 +79,8 @@ struct Args {
     int32_t tiles;
     uint32_t seed;
     float b1, omb1, b2, omb2, eps;
+    float minus_zero;
+    uint32_t zero;        // -1: eps is in [2^-60, 2^60], so that v = 0 needs no IEEE division; 0: it does
     Item t[N];
 };
 
@@ -124,17 +126,35 @@ __device__ __forceinline__ StepCoef step_coef(const Args<N>& a, const Item& t)
 
 // ---- eight values of a lane --------------------------------------------------------------------
 
+// 32 bytes, on a 32-byte boundary, in one access: a warp's accesses then cover whole sectors, which pairs of 16-byte
+// accesses at a stride of 32 do not (stores of half sectors took the read-out of 8-bit moments from 5.6 to 4.3 TB/s).
 __device__ __forceinline__ void load8(const float* p, float (&x)[8])
 {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7])
+                 : "l"(__cvta_generic_to_global(p)) : "memory");
 }
 
 __device__ __forceinline__ void store8(float* p, const float (&x)[8])
 {
-    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(__cvta_generic_to_global(p)), "f"(x[0]),
+                 "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7]) : "memory");
+}
+
+__device__ __forceinline__ void load8(const uint16_t* p, float (&x)[8])
+{
+    const uint4 a = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { x[2 * j] = u2f(w[j] << 16); x[2 * j + 1] = u2f(w[j] & 0xffff0000U); }
+}
+
+__device__ __forceinline__ void store8(uint16_t* p, const float (&x)[8])
+{
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = abx::pack_bf16_rne(x[2 * j], x[2 * j + 1]);
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // cnt valid values at p (0 beyond them); one vector where they are all there and aligned
@@ -151,10 +171,7 @@ __device__ __forceinline__ void load8(const float* p, int cnt, bool vec, float (
 __device__ __forceinline__ void load8(const uint16_t* p, int cnt, bool vec, float (&x)[8])
 {
     if (vec && cnt == 8) {
-        const uint4 a = *reinterpret_cast<const uint4*>(p);
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) { x[2 * j] = u2f(w[j] << 16); x[2 * j + 1] = u2f(w[j] & 0xffff0000U); }
+        load8(p, x);
     } else {
 #pragma unroll
         for (int k = 0; k < 8; ++k) x[k] = k < cnt ? u2f((uint32_t)p[k] << 16) : 0.0f;
@@ -173,59 +190,157 @@ __device__ __forceinline__ void store8(float* p, int cnt, bool vec, const float 
 
 __device__ __forceinline__ void store8(uint16_t* p, int cnt, bool vec, const float (&x)[8])
 {
-    uint32_t w[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] = abx::pack_bf16_rne(x[2 * j], x[2 * j + 1]);
     if (vec && cnt == 8) {
-        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        store8(p, x);
     } else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) if (k < cnt) p[k] = (uint16_t)(w[k >> 1] >> (16 * (k & 1)));
+        for (int k = 0; k < 8; ++k) if (k < cnt) p[k] = (uint16_t)abx::pack_bf16_rne(x[k], 0.0f);
     }
+}
+
+// ---- pairs -----------------------------------------------------------------------------------------
+// Two values per FP32 instruction, each rounded as the scalar instruction rounds it.
+
+using abx::f2x;
+using abx::fma2;
+using abx::mul2;
+using abx::pk2;
+using abx::up2;
+
+__device__ __forceinline__ f2x both(float x) { return pk2(x, x); }
+
+__device__ __forceinline__ f2x add2(f2x a, f2x b)
+{
+    f2x d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+// A product that an addition takes, rounded by itself: the assembler contracts mul.rn.f32x2 and add.rn.f32x2 into one
+// FMA (-fmad=false notwithstanding), but not an FMA whose third operand, -0, it cannot see: a kernel argument.
+__device__ __forceinline__ f2x term2(f2x a, f2x b, f2x minus_zero) { return fma2(a, b, minus_zero); }
+
+__device__ __forceinline__ f2x add2_down(f2x a, f2x b)
+{
+    f2x d;
+    asm("add.rm.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+__device__ __forceinline__ f2x sub2(f2x a, f2x b) { return fma2(b, both(-1.0f), a); }
+
+__device__ __forceinline__ void pairs(const float (&x)[8], f2x (&p)[4])
+{
+#pragma unroll
+    for (int j = 0; j < 4; ++j) p[j] = pk2(x[2 * j], x[2 * j + 1]);
+}
+
+__device__ __forceinline__ void singles(const f2x (&p)[4], float (&x)[8])
+{
+#pragma unroll
+    for (int j = 0; j < 4; ++j) up2(p[j], x[2 * j], x[2 * j + 1]);
+}
+
+// the first n of a pair, 0 for the others
+__device__ __forceinline__ f2x first_of(f2x x, int n)
+{
+    float a, b;
+    up2(x, a, b);
+    return pk2(n > 0 ? a : 0.0f, n > 1 ? b : 0.0f);
+}
+
+// Root and quotient by Newton's iteration from the hardware's approximations, with Markstein's last step: the exact
+// remainder by FMA, times the reciprocal, added to the approximation, rounds correctly (P. Markstein, IBM J. Res.
+// Dev. 34(1), 1990).  In pairs that is a third of the instructions of the scalar IEEE operations, which otherwise
+// take a quarter of the kernel.  The root equals __fsqrt_rn for every float of [2^-100, 2^120) and for 0; the
+// quotient equalled __fdiv_rn for 7.7e10 random operands, |x| above 2^-100 and the divisor in [2^-60, 2^90].
+// Outside (see `plain` in step_kernel) the IEEE operations are used.
+__device__ __forceinline__ f2x sqrt2(f2x x)
+{
+    float a, b, ya, yb;
+    up2(x, a, b);
+    asm("rsqrt.approx.f32 %0, %1;" : "=f"(ya) : "f"(fmaxf(a, 0x1p-120f)));
+    asm("rsqrt.approx.f32 %0, %1;" : "=f"(yb) : "f"(fmaxf(b, 0x1p-120f)));
+    const f2x y = pk2(ya, yb), s = mul2(x, y), h = mul2(y, both(0.5f));
+    return fma2(fma2(mul2(s, both(-1.0f)), s, x), h, s);
+}
+
+__device__ __forceinline__ f2x quotient2(f2x x, f2x d)
+{
+    float a, b, ya, yb;
+    up2(d, a, b);
+    asm("rcp.approx.f32 %0, %1;" : "=f"(ya) : "f"(a));
+    asm("rcp.approx.f32 %0, %1;" : "=f"(yb) : "f"(b));
+    const f2x n = mul2(d, both(-1.0f)), y0 = pk2(ya, yb);
+    const f2x y = fma2(y0, fma2(n, y0, both(1.0f)), y0);
+    const f2x q = mul2(x, y);
+    return fma2(fma2(n, q, x), y, q);
 }
 
 // ---- the 8-bit block format ----------------------------------------------------------------------
 
 // Bytes become floats by way of the significand of 2^23 + byte: one byte permute and one exact subtraction each.
-__device__ __forceinline__ void decode_m(uint2 codes, float s, float (&x)[8])
+__device__ __forceinline__ f2x bytes2(uint32_t w, int k)
+{
+    return pk2(u2f(__byte_perm(w, 0x4b000000U, 0x7440 + k)), u2f(__byte_perm(w, 0x4b000000U, 0x7441 + k)));
+}
+
+__device__ __forceinline__ void decode_m(uint2 codes, float s, f2x (&m)[4])
 {
     const uint32_t w[2] = {codes.x ^ 0x80808080U, codes.y ^ 0x80808080U};   // code + 128
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-        x[k] = __fmul_rn(u2f(__byte_perm(w[k >> 2], 0x4b000000U, 0x7440 + (k & 3))) - (8388608.0f + 128.0f), s);
+    for (int j = 0; j < 4; ++j) m[j] = mul2(add2(bytes2(w[j >> 1], 2 * (j & 1)), both(-8388736.0f)), both(s));
 }
 
-__device__ __forceinline__ void decode_v(uint2 codes, float s, float (&x)[8])
+__device__ __forceinline__ void decode_v(uint2 codes, float s, f2x (&v)[4])
 {
     const uint32_t w[2] = {codes.x, codes.y};
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const float r = __fmul_rn(u2f(__byte_perm(w[k >> 2], 0x4b000000U, 0x7440 + (k & 3))) - 8388608.0f, s);
-        x[k] = __fmul_rn(r, r);
+    for (int j = 0; j < 4; ++j) {
+        const f2x r = mul2(add2(bytes2(w[j >> 1], 2 * (j & 1)), both(-8388608.0f)), both(s));
+        v[j] = mul2(r, r);
     }
 }
 
 // The block's largest magnitude; a NaN's bits are above every number's, so it is a NaN if any value is.
-__device__ __forceinline__ float block_max(const float (&x)[8])
+__device__ __forceinline__ float block_max(const f2x (&x)[4])
 {
     uint32_t m = 0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) m = max(m, f2u(x[k]) & 0x7fffffffU);
+    for (int j = 0; j < 4; ++j) {
+        float a, b;
+        up2(x[j], a, b);
+        m = __vimax3_u32(m, f2u(a) & 0x7fffffffU, f2u(b) & 0x7fffffffU);
+    }
     return u2f(__reduce_max_sync(0xffffffffU, m));
 }
 
-// The factor from values to codes and the stored scale.  `below` is the float next below the largest code: value
-// * (below / top) then never rounds above that code.  A block under 2^-100 is stored as zeros: below / top would
-// overflow.  top not finite: the stored scale is NaN.
-__device__ __forceinline__ float block_scale(float top, float below, float inverse, float& scale)
+constexpr float kBelow127 = 126.99999237060546875f, kBelow255 = 254.9999847412109375f;
+
+struct BlockScales {
+    float to_m, to_root;   // from values to codes
+    float m, root;         // stored
+};
+
+// The numerators are the floats next below the largest codes: value * (below / top) then never rounds above that code.
+// A block under 2^-100 is stored as zeros: below / top could overflow.  top not finite: the stored scale is NaN.
+__device__ __forceinline__ BlockScales block_scales(float top_m, float top_root)
 {
-    const bool some = !(top <= 0x1p-100f);
-    scale = some ? __fmul_rn(top, inverse) : 0.0f;
-    if (!(top <= 3.402823466e38f)) scale = u2f(0x7fffffffU);
-    return some ? __fdiv_rn(below, top) : 0.0f;
+    constexpr float kLeast = 0x1p-100f, kMost = 3.402823466e38f;
+    BlockScales s;
+    if (top_m >= 0x1p-60f && top_m <= 0x1p90f && top_root >= 0x1p-60f && top_root <= 0x1p90f) {
+        up2(quotient2(pk2(kBelow127, kBelow255), pk2(top_m, top_root)), s.to_m, s.to_root);
+        s.m = __fmul_rn(top_m, 1.0f / 127.0f);
+        s.root = __fmul_rn(top_root, 1.0f / 255.0f);
+        return s;
+    }
+    s.to_m = top_m <= kLeast ? 0.0f : __fdiv_rn(kBelow127, top_m);
+    s.to_root = top_root <= kLeast ? 0.0f : __fdiv_rn(kBelow255, top_root);
+    s.m = top_m <= kLeast ? 0.0f : top_m <= kMost ? __fmul_rn(top_m, 1.0f / 127.0f) : u2f(0x7fffffffU);
+    s.root = top_root <= kLeast ? 0.0f : top_root <= kMost ? __fmul_rn(top_root, 1.0f / 255.0f) : u2f(0x7fffffffU);
+    return s;
 }
 
-constexpr float kBelow127 = 126.99999237060546875f, kBelow255 = 254.9999847412109375f;
 constexpr float kWhole = 12582912.0f;   // 1.5 * 2^23: a sum with it has the addend, rounded, in its low bits
 
 __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d)
@@ -233,40 +348,55 @@ __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, ui
     return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
-template <bool SR>
-__device__ __forceinline__ uint2 encode_m(const float (&m)[8], float f, const uint32_t (&r)[8])
+// 16 random bits as a float of [0, 1): 2^23 + bits, scaled and shifted in one exact FMA.
+template <int HIGH>
+__device__ __forceinline__ f2x uniform2(uint32_t r0, uint32_t r1)
 {
-    uint32_t q[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const float x = __fmul_rn(m[k], f);
-        if (SR) {   // floor(x + u), u = the low 16 bits / 2^16
-            const float u = __fmul_rn(u2f(0x4b000000U | (r[k] & 0xffffU)) - 8388608.0f, 0x1p-16f);
-            q[k] = f2u(__fadd_rd(__fadd_rn(x, u), kWhole));
-        } else {
-            q[k] = f2u(__fadd_rn(x, kWhole));
-        }
-    }
-    return make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
+    const f2x x = pk2(u2f(__byte_perm(r0, 0x4b000000U, HIGH ? 0x7432 : 0x7410)),
+                      u2f(__byte_perm(r1, 0x4b000000U, HIGH ? 0x7432 : 0x7410)));
+    return fma2(x, both(0x1p-16f), both(-128.0f));
 }
 
 template <bool SR>
-__device__ __forceinline__ uint2 encode_v(const float (&root)[8], float f, const uint32_t (&r)[8])
+__device__ __forceinline__ uint2 encode_m(const f2x (&m)[4], float f, const uint32_t (&r)[8], f2x minus_zero)
+{
+    float q[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const f2x x = term2(m[j], both(f), minus_zero);
+        const f2x z = SR ? add2_down(add2(x, uniform2<0>(r[2 * j], r[2 * j + 1])), both(kWhole))   // floor(x + u)
+                         : add2(x, both(kWhole));
+        up2(z, q[2 * j], q[2 * j + 1]);
+    }
+    return make_uint2(pack4(f2u(q[0]), f2u(q[1]), f2u(q[2]), f2u(q[3])), pack4(f2u(q[4]), f2u(q[5]), f2u(q[6]), f2u(q[7])));
+}
+
+template <bool SR>
+__device__ __forceinline__ uint2 encode_v(const f2x (&root)[4], float f, const uint32_t (&r)[8])
 {
     uint32_t c[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const float x = __fmul_rn(root[k], f);
+    for (int j = 0; j < 4; ++j) {
+        // below 1 a positive root counts as 1 (saturate gives 0 for 0 and 1 for every root of a positive float)
+        float ra, rb, xa, xb, za, zb;
+        up2(root[j], ra, rb);
+        up2(mul2(root[j], both(f)), xa, xb);
+        const f2x x = pk2(fmaxf(xa, __saturatef(ra * 0x1p100f)), fmaxf(xb, __saturatef(rb * 0x1p100f)));
         if (SR) {
-            const float z = __fadd_rd(x, kWhole);
-            const float q = z - kWhole;
-            const float u = __fmul_rn(u2f(__byte_perm(r[k], 0x4b000000U, 0x7632)) - 8388608.0f, 0x1p-16f);
-            const bool up = __fmul_rn(x - q, x + q) > __fmul_rn(u, q + q + 1.0f);
-            c[k] = (f2u(z) & 0xffU) + (up ? 1U : 0U);
+            const f2x z = add2_down(x, both(kWhole)), q = add2(z, both(-kWhole));
+            const f2x part = mul2(sub2(x, q), add2(x, q));
+            const f2x step = mul2(uniform2<1>(r[2 * j], r[2 * j + 1]), fma2(q, both(2.0f), both(1.0f)));
+            float pa, pb, sa, sb;
+            up2(z, za, zb);
+            up2(part, pa, pb);
+            up2(step, sa, sb);
+            c[2 * j] = f2u(za) + (pa > sa ? 1U : 0U);
+            c[2 * j + 1] = f2u(zb) + (pb > sb ? 1U : 0U);
         } else {
-            c[k] = f2u(__fadd_rn(x, kWhole)) & 0xffU;
+            up2(add2(x, both(kWhole)), za, zb);
+            c[2 * j] = f2u(za);
+            c[2 * j + 1] = f2u(zb);
         }
-        c[k] = root[k] > 0.0f ? max(c[k], 1U) : c[k];
     }
     return make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
 }
@@ -284,84 +414,162 @@ __device__ __forceinline__ int find_item(const Args<N>& a, int tile)
     return lo;
 }
 
-// W: the weights' and gradients' type (float, or uint16_t for bf16 bits with an fp32 master).
+// Which tensor a tile belongs to, for tiles that only go up.
+template <int N>
+struct Cursor {
+    int item;
+    __device__ __forceinline__ explicit Cursor(const Args<N>& a, int tile) : item(find_item(a, tile)) {}
+    __device__ __forceinline__ const Item& at(const Args<N>& a, int tile)
+    {
+        while (item + 1 < a.count && a.t[item + 1].tile_begin <= tile) ++item;
+        return a.t[item];
+    }
+};
+
+// What the blocks of a tile share: the tensor's arrays at the tile's first element.  All of it is the same for every
+// thread, so that an access is a uniform address plus a thread's own fixed offset.
+template <typename W>
+struct Tile {
+    W* w;
+    const W* g;
+    float* master;
+    uint8_t* m;
+    uint8_t* v;
+    float* m_scale;
+    float* v_scale;
+    uint32_t place;   // the first element's (low 32 bits), which the rounding's random words go by
+};
+
+struct Constants {
+    float scale, b1, omb1, b2, omb2, eps;
+    f2x minus_zero;
+    uint32_t zero;
+};
+
+// One block: 8 values per lane, `cnt` of them valid (8 in a whole tile, where FULL).
+template <bool I8, bool SR, bool FULL, typename W>
+__device__ __forceinline__ void update(const Tile<W>& t, const Constants& k, const StepCoef& c, int cnt, bool vec)
+{
+    constexpr bool kMaster = sizeof(W) == 2;
+    const uint32_t own = threadIdx.x * 8, block = threadIdx.x / 32;
+    const f2x nz = k.minus_zero;
+    float x[8];
+    f2x g[4], p[4], m[4], v[4], root[4], q[4];
+    if constexpr (FULL) load8(t.g + own, x);
+    else load8(t.g + own, cnt, vec, x);
+    pairs(x, g);
+    if constexpr (kMaster) load8(t.master + own, x);
+    else if constexpr (FULL) load8(t.w + own, x);
+    else load8(t.w + own, cnt, vec, x);
+    pairs(x, p);
+    if constexpr (I8) {
+        const uint2 mc = *reinterpret_cast<const uint2*>(t.m + own), vc = *reinterpret_cast<const uint2*>(t.v + own);
+        decode_m(mc, t.m_scale[block], m);
+        decode_v(vc, t.v_scale[block], v);
+    } else {
+        load8(reinterpret_cast<const float*>(t.m) + own, x);
+        pairs(x, m);
+        load8(reinterpret_cast<const float*>(t.v) + own, x);
+        pairs(x, v);
+    }
+    // `low`, `high`: the extremes of v's bits, a zero left out where eps alone is a divisor that quotient2 takes
+    uint32_t low = 0xffffffffU, high = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const f2x gj = mul2(g[j], both(k.scale));
+        m[j] = add2(term2(m[j], both(k.b1), nz), term2(gj, both(k.omb1), nz));
+        v[j] = add2(term2(v[j], both(k.b2), nz), term2(mul2(gj, both(k.omb2)), gj, nz));
+        float v0, v1;
+        up2(v[j], v0, v1);
+        low = __viaddmin_u32(f2u(v0), k.zero, __viaddmin_u32(f2u(v1), k.zero, low));
+        high = __vimax3_u32(high, f2u(v0), f2u(v1));
+        root[j] = sqrt2(v[j]);
+        q[j] = quotient2(m[j], add2(term2(root[j], both(c.inv_sqrt_bc2), nz), both(k.eps)));
+    }
+    const bool plain = low < 0x0dffffffU || high >= 0x7b800000U;   // under 2^-99 or not under 2^120
+    if (__builtin_expect(plain, 0)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float v0, v1, m0, m1;
+            up2(v[j], v0, v1);
+            up2(m[j], m0, m1);
+            v0 = __fsqrt_rn(v0);
+            v1 = __fsqrt_rn(v1);
+            root[j] = pk2(v0, v1);
+            q[j] = pk2(__fdiv_rn(m0, __fadd_rn(__fmul_rn(v0, c.inv_sqrt_bc2), k.eps)),
+                       __fdiv_rn(m1, __fadd_rn(__fmul_rn(v1, c.inv_sqrt_bc2), k.eps)));
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) p[j] = sub2(term2(p[j], both(c.decay), nz), term2(q[j], both(c.step_size), nz));
+    if constexpr (!FULL) {   // beyond the tensor's end the state stays zero
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            p[j] = first_of(p[j], cnt - 2 * j);
+            m[j] = first_of(m[j], cnt - 2 * j);
+            root[j] = first_of(root[j], cnt - 2 * j);
+        }
+    }
+    singles(p, x);
+    if constexpr (kMaster) store8(t.master + own, x);
+    if constexpr (FULL) store8(t.w + own, x);
+    else store8(t.w + own, cnt, vec, x);
+    if constexpr (I8) {
+        uint32_t r[8];
+        if constexpr (SR) {
+            uint32_t r0[4], r1[4];
+            abx::hash4(t.place + own, c.stream, r0);
+            abx::hash4(t.place + own + 4, c.stream, r1);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { r[i] = r0[i]; r[4 + i] = r1[i]; }
+        }
+        const BlockScales s = block_scales(block_max(m), block_max(root));
+        *reinterpret_cast<uint2*>(t.m + own) = encode_m<SR>(m, s.to_m, r, nz);
+        *reinterpret_cast<uint2*>(t.v + own) = encode_v<SR>(root, s.to_root, r);
+        if (threadIdx.x % 32 == 0) {
+            t.m_scale[block] = s.m;
+            t.v_scale[block] = s.root;
+        }
+    } else {
+        singles(m, x);
+        store8(reinterpret_cast<float*>(t.m) + own, x);
+        singles(v, x);
+        store8(reinterpret_cast<float*>(t.v) + own, x);
+    }
+}
+
+// W: the weights' and gradients' type (float, or uint16_t for bf16 bits with an fp32 master).  A warp takes one block
+// of each of its CTA's tiles.
 template <bool I8, bool SR, typename W, int N>
 __global__ void __launch_bounds__(kThreads) step_kernel(const __grid_constant__ Args<N> a)
 {
-    constexpr bool kMaster = sizeof(W) == 2;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __shared__ bool last;
     // skip is a flag as loss scalers write it; a norm that is not finite says the same of the gradients
     if (a.skip != nullptr && !(*a.skip == 0.0f)) return;
     if (a.norm != nullptr && !(fabsf(*a.norm) <= 3.402823466e38f)) return;
-    const float scale = a.g_scale != nullptr ? *a.g_scale : 1.0f;
+    const Constants k{a.g_scale != nullptr ? *a.g_scale : 1.0f, a.b1, a.omb1, a.b2, a.omb2, a.eps, both(a.minus_zero), a.zero};
     StepCoef c;
     int current = -1;
+    Cursor<N> now(a, blockIdx.x);
     for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
-        const int it = find_item(a, tile);
-        const Item& t = a.t[it];
-        if (it != current) {
+        const Item& t = now.at(a, tile);
+        if (now.item != current) {
             c = step_coef(a, t);
-            current = it;
+            current = now.item;
         }
+        constexpr int kMoment = I8 ? 1 : 4;   // bytes
+        const int64_t at = (int64_t)(tile - t.tile_begin) * kTile, left = t.n - at;
+        const Tile<W> here{static_cast<W*>(t.w) + at, static_cast<const W*>(t.g) + at, t.master + at,
+                           static_cast<uint8_t*>(t.m) + at * kMoment, static_cast<uint8_t*>(t.v) + at * kMoment,
+                           t.m_scale + at / kBlock, t.v_scale + at / kBlock, (uint32_t)at};
         const bool vec = t.index_vec & 1;
-        const int64_t b0 = (int64_t)(tile - t.tile_begin) * kTile + warp * kBlock;
-        if (b0 >= t.n) continue;
-        const int64_t i0 = b0 + lane * 8;
-        const int64_t left = t.n - i0;
-        const int cnt = left >= 8 ? 8 : (left > 0 ? (int)left : 0);
-
-        float g[8], p[8], m[8], v[8], root[8];
-        load8(static_cast<const W*>(t.g) + i0, cnt, vec, g);
-        if constexpr (kMaster) load8(t.master + i0, p);
-        else load8(static_cast<const float*>(t.w) + i0, cnt, vec, p);
-        if constexpr (I8) {
-            const uint2 mc = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(t.m) + i0);
-            const uint2 vc = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(t.v) + i0);
-            decode_m(mc, t.m_scale[b0 / kBlock], m);
-            decode_v(vc, t.v_scale[b0 / kBlock], v);
-        } else {
-            load8(static_cast<const float*>(t.m) + i0, m);
-            load8(static_cast<const float*>(t.v) + i0, v);
-        }
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const float gk = __fmul_rn(g[k], scale);
-            m[k] = __fadd_rn(__fmul_rn(m[k], a.b1), __fmul_rn(gk, a.omb1));
-            v[k] = __fadd_rn(__fmul_rn(v[k], a.b2), __fmul_rn(__fmul_rn(gk, a.omb2), gk));
-            root[k] = __fsqrt_rn(v[k]);
-            const float d = __fadd_rn(__fmul_rn(root[k], c.inv_sqrt_bc2), a.eps);
-            p[k] = __fsub_rn(__fmul_rn(p[k], c.decay), __fmul_rn(__fdiv_rn(m[k], d), c.step_size));
-        }
-        if (cnt < 8) {   // beyond the tensor's end the state stays zero
-#pragma unroll
-            for (int k = 0; k < 8; ++k) if (k >= cnt) p[k] = m[k] = root[k] = 0.0f;
-        }
-        if constexpr (kMaster) store8(t.master + i0, p);
-        store8(static_cast<W*>(t.w) + i0, cnt, vec, p);
-        if constexpr (I8) {
-            uint32_t r[8];
-            if constexpr (SR) {
-                uint32_t r0[4], r1[4];
-                abx::hash4((uint32_t)i0, c.stream, r0);
-                abx::hash4((uint32_t)i0 + 4, c.stream, r1);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) { r[k] = r0[k]; r[4 + k] = r1[k]; }
-            }
-            float sm, sv;
-            const float fm = block_scale(block_max(m), kBelow127, 1.0f / 127.0f, sm);
-            const float fv = block_scale(block_max(root), kBelow255, 1.0f / 255.0f, sv);
-            *reinterpret_cast<uint2*>(static_cast<uint8_t*>(t.m) + i0) = encode_m<SR>(m, fm, r);
-            *reinterpret_cast<uint2*>(static_cast<uint8_t*>(t.v) + i0) = encode_v<SR>(root, fv, r);
-            if (lane == 0) {
-                t.m_scale[b0 / kBlock] = sm;
-                t.v_scale[b0 / kBlock] = sv;
-            }
-        } else {
-            store8(static_cast<float*>(t.m) + i0, m);
-            store8(static_cast<float*>(t.v) + i0, v);
+        if (vec && left >= kTile) {
+            update<I8, SR, true, W>(here, k, c, 8, true);
+        } else if (threadIdx.x / 32 * kBlock < left) {
+            const int cnt = (int)(left < kTile ? left : kTile) - (int)threadIdx.x * 8;
+            update<I8, SR, false, W>(here, k, c, cnt < 0 ? 0 : cnt > 8 ? 8 : cnt, vec);
         }
     }
-    __shared__ bool last;
     __syncthreads();                      // this CTA has read its step counts
     if (threadIdx.x == 0) {
         __threadfence();
@@ -382,21 +590,37 @@ struct I8Args {
     float* values;
     int64_t n;
     int64_t blocks;
+    float minus_zero;
 };
 
+// A warp takes four blocks at a time, so that enough loads are under way.
 template <bool V>
 __global__ void __launch_bounds__(kThreads) i8_decode(const I8Args a)
 {
+    constexpr int kAtOnce = 4;
     const int lane = threadIdx.x & 31;
-    const bool vec = (reinterpret_cast<uintptr_t>(a.values) & 15) == 0;
-    for (int64_t b = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5); b < a.blocks; b += (int64_t)gridDim.x * kWarps) {
-        const int64_t i0 = b * kBlock + lane * 8, left = a.n - i0;
-        if (left <= 0) continue;
-        const uint2 c = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.codes) + i0);
-        float x[8];
-        if constexpr (V) decode_v(c, a.scales[b], x);
-        else decode_m(c, a.scales[b], x);
-        store8(a.values + i0, left < 8 ? (int)left : 8, vec, x);
+    const bool vec = (reinterpret_cast<uintptr_t>(a.values) & 31) == 0;
+    const int64_t stride = (int64_t)gridDim.x * kWarps * kAtOnce;
+    for (int64_t b = ((int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5)) * kAtOnce; b < a.blocks; b += stride) {
+        uint2 c[kAtOnce];
+        float s[kAtOnce];
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j)
+            if (b + j < a.blocks) {
+                c[j] = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.codes) + (b + j) * kBlock + lane * 8);
+                s[j] = a.scales[b + j];
+            }
+#pragma unroll
+        for (int j = 0; j < kAtOnce; ++j) {
+            const int64_t i0 = (b + j) * kBlock + lane * 8, left = a.n - i0;
+            if (b + j >= a.blocks || left <= 0) break;
+            float x[8];
+            f2x y[4];
+            if constexpr (V) decode_v(c[j], s[j], y);
+            else decode_m(c[j], s[j], y);
+            singles(y, x);
+            store8(a.values + i0, left < 8 ? (int)left : 8, vec, x);
+        }
     }
 }
 
@@ -405,7 +629,7 @@ template <bool V>
 __global__ void __launch_bounds__(kThreads) i8_encode(const I8Args a)
 {
     const int lane = threadIdx.x & 31;
-    const bool vec = (reinterpret_cast<uintptr_t>(a.values) & 15) == 0;
+    const bool vec = (reinterpret_cast<uintptr_t>(a.values) & 31) == 0;
     for (int64_t b = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5); b < a.blocks; b += (int64_t)gridDim.x * kWarps) {
         const int64_t i0 = b * kBlock + lane * 8, left = a.n - i0;
         float x[8];
@@ -414,13 +638,16 @@ __global__ void __launch_bounds__(kThreads) i8_encode(const I8Args a)
 #pragma unroll
             for (int k = 0; k < 8; ++k) x[k] = __fsqrt_rn(x[k] < 0.0f ? 0.0f : x[k]);
         }
-        uint32_t none[8] = {};
-        float s;
+        const uint32_t none[8] = {};
+        f2x y[4];
+        pairs(x, y);
+        const float top = block_max(y);
+        const BlockScales s = block_scales(top, top);
         uint2 c;
-        if constexpr (V) c = encode_v<false>(x, block_scale(block_max(x), kBelow255, 1.0f / 255.0f, s), none);
-        else c = encode_m<false>(x, block_scale(block_max(x), kBelow127, 1.0f / 127.0f, s), none);
+        if constexpr (V) c = encode_v<false>(y, s.to_root, none);
+        else c = encode_m<false>(y, s.to_m, none, both(a.minus_zero));
         *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.codes) + i0) = c;
-        if (lane == 0) a.scales[b] = s;
+        if (lane == 0) a.scales[b] = V ? s.root : s.m;
     }
 }
 
@@ -438,7 +665,7 @@ int check(const abx_graph_tensor& t, const abx_graph_step& h)
     if (h.moments == ABX_DT_I8 && (!t.m_scale || !t.v_scale)) return ABX_E_SCALE_NULL;
     const uintptr_t es = t.dtype == ABX_DT_BF16 ? 2 : 4;
     if (off(t.w, es) || off(t.g, es) || off(t.step, 8)) return ABX_E_ALIGN;
-    if (off(t.m, 16) || off(t.v, 16) || (t.dtype == ABX_DT_BF16 && off(t.master, 16))) return ABX_E_ALIGN;
+    if (off(t.m, 32) || off(t.v, 32) || (t.dtype == ABX_DT_BF16 && off(t.master, 32))) return ABX_E_ALIGN;
     if (h.moments == ABX_DT_I8 && (off(t.m_scale, 4) || off(t.v_scale, 4))) return ABX_E_ALIGN;
     return ABX_OK;
 }
@@ -481,10 +708,13 @@ int run_batch(const abx_graph_tensor* t, const int32_t* order, int32_t count, in
     a.b1 = (float)h.beta1; a.omb1 = (float)(1.0 - h.beta1);
     a.b2 = (float)h.beta2; a.omb2 = (float)(1.0 - h.beta2);
     a.eps = (float)h.eps;
+    a.minus_zero = -0.0f;
+    a.zero = a.eps >= 0x1p-60f && a.eps <= 0x1p60f ? 0xffffffffU : 0U;
     int64_t next = 0;
     for (int32_t j = 0; j < count; ++j) {
         const abx_graph_tensor& s = t[order[j]];
-        const uint32_t vec = !off(s.w, 16) && !off(s.g, 16);
+        const uintptr_t wide = s.dtype == ABX_DT_F32 ? 32 : 16;   // bytes of 8 values
+        const uint32_t vec = !off(s.w, wide) && !off(s.g, wide);
         a.t[j] = Item{s.w, s.g, s.master, s.m, s.v, s.m_scale, s.v_scale, s.step, s.n, (int32_t)next, s.index << 1 | vec};
         next += (s.n + kTile - 1) / kTile;
     }
@@ -507,14 +737,14 @@ int i8_check(const void* codes, const float* scales, const float* values, int64_
 }
 
 template <void (*KM)(const I8Args), void (*KV)(const I8Args)>
-int i8_run(void* stream, void* codes, float* scales, float* values, int64_t n, int32_t role, const char* what)
+int i8_run(void* stream, void* codes, float* scales, float* values, int64_t n, int32_t role, int at_once, const char* what)
 {
     if (int rc = i8_check(codes, scales, values, n, role)) return rc;
     if (n == 0) return ABX_OK;
-    const I8Args a{codes, scales, values, n, (n + kBlock - 1) / kBlock};
+    const I8Args a{codes, scales, values, n, (n + kBlock - 1) / kBlock, -0.0f};
     int grid = 0;
     if (int rc = resident_ctas(role ? (const void*)KV : (const void*)KM, &grid)) return rc;
-    const int64_t need = (a.blocks + kWarps - 1) / kWarps;
+    const int64_t need = (a.blocks + kWarps * at_once - 1) / (kWarps * at_once);
     if (need < grid) grid = (int)need;
     if (role) KV<<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
     else KM<<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
@@ -567,11 +797,11 @@ ABX_API int abx_graph_adamw(void* stream, const abx_graph_tensor* tensors, int32
 ABX_API int abx_i8_decode(void* stream, const void* codes, const float* scales, float* values, int64_t n, int32_t role)
 {
     return i8_run<i8_decode<false>, i8_decode<true>>(stream, const_cast<void*>(codes), const_cast<float*>(scales), values,
-                                                     n, role, "i8_decode launch");
+                                                     n, role, 4, "i8_decode launch");
 }
 
 ABX_API int abx_i8_encode(void* stream, const float* values, void* codes, float* scales, int64_t n, int32_t role)
 {
-    return i8_run<i8_encode<false>, i8_encode<true>>(stream, codes, scales, const_cast<float*>(values), n, role,
+    return i8_run<i8_encode<false>, i8_encode<true>>(stream, codes, scales, const_cast<float*>(values), n, role, 1,
                                                      "i8_encode launch");
 }

@@ -282,7 +282,7 @@ int abx_convert(void* stream, const abx_state* src, const abx_state* dst, int64_
  * captured the call performs the next step at every replay. */
 
 /* One tensor.  m, v, the scales and master are padded to whole ABX_I8_BLOCK blocks (the
- * padding stays zero) and start on 16-byte boundaries (the scales on 4-byte ones). */
+ * padding stays zero) and start on 32-byte boundaries (the scales on 4-byte ones). */
 typedef struct abx_graph_tensor {
     void* w;            /* the weights, dtype; fp32 weights are their own master */
     const void* g;      /* the gradient, dtype */
