@@ -44,6 +44,9 @@ using abx::u2f;
 constexpr int kBlock = ABX_I8_BLOCK;      // values per scale: 8 per lane of a warp
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
+// Resident CTAs per SM: at most 96 registers per thread with 8-bit moments (6 CTAs and 80 registers were as fast, 7
+// spilled: 654, 659, 725 us for 202M parameters), 64 with fp32 ones (23 against 28 us for 184 small tensors at 5).
+template <bool I8> constexpr int kStepCtas = I8 ? 5 : 8;
 constexpr int kTile = kWarps * kBlock;    // elements of one tensor that a CTA takes at a time
 constexpr int kMany = 384;                // tensors per launch: the parameter block stays under 32764 bytes
 constexpr int kFew = 24;                  // ... of the variant for few tensors (a smaller block to pass)
@@ -80,7 +83,7 @@ struct Args {
     uint32_t seed;
     float b1, omb1, b2, omb2, eps;
     float minus_zero;
-    uint32_t zero;        // -1: eps is in [2^-60, 2^60], so that v = 0 needs no IEEE division; 0: it does
+    uint32_t zero_is_plain;   // eps is in [2^-60, 2^60]: v = 0 needs no IEEE division
     Item t[N];
 };
 
@@ -258,11 +261,14 @@ __device__ __forceinline__ f2x first_of(f2x x, int n)
 __device__ __forceinline__ f2x sqrt2(f2x x)
 {
     float a, b, ya, yb;
-    up2(x, a, b);
-    asm("rsqrt.approx.f32 %0, %1;" : "=f"(ya) : "f"(fmaxf(a, 0x1p-120f)));
-    asm("rsqrt.approx.f32 %0, %1;" : "=f"(yb) : "f"(fmaxf(b, 0x1p-120f)));
+    up2(add2(x, both(0x1p-126f)), a, b);   // no change above 2^-100, and a finite reciprocal root of 0
+    asm("rsqrt.approx.f32 %0, %1;" : "=f"(ya) : "f"(a));
+    asm("rsqrt.approx.f32 %0, %1;" : "=f"(yb) : "f"(b));
     const f2x y = pk2(ya, yb), s = mul2(x, y), h = mul2(y, both(0.5f));
-    return fma2(fma2(mul2(s, both(-1.0f)), s, x), h, s);
+    float sa, sb;
+    up2(x, a, b);
+    up2(s, sa, sb);
+    return fma2(pk2(__fmaf_rn(-sa, sa, a), __fmaf_rn(-sb, sb, b)), h, s);
 }
 
 __device__ __forceinline__ f2x quotient2(f2x x, f2x d)
@@ -305,14 +311,14 @@ __device__ __forceinline__ void decode_v(uint2 codes, float s, f2x (&v)[4])
 // The block's largest magnitude; a NaN's bits are above every number's, so it is a NaN if any value is.
 __device__ __forceinline__ float block_max(const f2x (&x)[4])
 {
-    uint32_t m = 0;
+    float m = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         float a, b;
         up2(x[j], a, b);
-        m = __vimax3_u32(m, f2u(a) & 0x7fffffffU, f2u(b) & 0x7fffffffU);
+        asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(m), "f"(a), "f"(b));
     }
-    return u2f(__reduce_max_sync(0xffffffffU, m));
+    return u2f(__reduce_max_sync(0xffffffffU, f2u(m)));
 }
 
 constexpr float kBelow127 = 126.99999237060546875f, kBelow255 = 254.9999847412109375f;
@@ -371,34 +377,40 @@ __device__ __forceinline__ uint2 encode_m(const f2x (&m)[4], float f, const uint
     return make_uint2(pack4(f2u(q[0]), f2u(q[1]), f2u(q[2]), f2u(q[3])), pack4(f2u(q[4]), f2u(q[5]), f2u(q[6]), f2u(q[7])));
 }
 
+// Codes of which those that are 0 become 1, but for the bytes that are 1 in `zeros`: code 0 is for 0 alone.
+__device__ __forceinline__ uint32_t at_least_one(uint32_t codes, uint32_t zeros)
+{
+    // the sign bits of 0 bytes; a borrow also marks a byte of 1 above one, which keeps its value
+    const uint32_t none = (codes - 0x01010101U) & ~codes & 0x80808080U;
+    return codes | (none >> 7 & ~zeros);
+}
+
 template <bool SR>
-__device__ __forceinline__ uint2 encode_v(const f2x (&root)[4], float f, const uint32_t (&r)[8])
+__device__ __forceinline__ uint2 encode_v(const f2x (&root)[4], float f, const uint32_t (&r)[8], const uint32_t (&zeros)[2],
+                                          f2x minus_zero)
 {
     uint32_t c[8];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        // below 1 a positive root counts as 1 (saturate gives 0 for 0 and 1 for every root of a positive float)
-        float ra, rb, xa, xb, za, zb;
-        up2(root[j], ra, rb);
-        up2(mul2(root[j], both(f)), xa, xb);
-        const f2x x = pk2(fmaxf(xa, __saturatef(ra * 0x1p100f)), fmaxf(xb, __saturatef(rb * 0x1p100f)));
+        float za, zb;
+        const f2x x = term2(root[j], both(f), minus_zero);
         if (SR) {
             const f2x z = add2_down(x, both(kWhole)), q = add2(z, both(-kWhole));
             const f2x part = mul2(sub2(x, q), add2(x, q));
             const f2x step = mul2(uniform2<1>(r[2 * j], r[2 * j + 1]), fma2(q, both(2.0f), both(1.0f)));
-            float pa, pb, sa, sb;
+            float da, db;
             up2(z, za, zb);
-            up2(part, pa, pb);
-            up2(step, sa, sb);
-            c[2 * j] = f2u(za) + (pa > sa ? 1U : 0U);
-            c[2 * j + 1] = f2u(zb) + (pb > sb ? 1U : 0U);
+            up2(sub2(step, part), da, db);   // negative: up
+            c[2 * j] = f2u(za) + (f2u(da) >> 31);
+            c[2 * j + 1] = f2u(zb) + (f2u(db) >> 31);
         } else {
             up2(add2(x, both(kWhole)), za, zb);
             c[2 * j] = f2u(za);
             c[2 * j + 1] = f2u(zb);
         }
     }
-    return make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
+    return make_uint2(at_least_one(pack4(c[0], c[1], c[2], c[3]), zeros[0]),
+                      at_least_one(pack4(c[4], c[5], c[6], c[7]), zeros[1]));
 }
 
 // ---- the step ------------------------------------------------------------------------------------
@@ -414,20 +426,8 @@ __device__ __forceinline__ int find_item(const Args<N>& a, int tile)
     return lo;
 }
 
-// Which tensor a tile belongs to, for tiles that only go up.
-template <int N>
-struct Cursor {
-    int item;
-    __device__ __forceinline__ explicit Cursor(const Args<N>& a, int tile) : item(find_item(a, tile)) {}
-    __device__ __forceinline__ const Item& at(const Args<N>& a, int tile)
-    {
-        while (item + 1 < a.count && a.t[item + 1].tile_begin <= tile) ++item;
-        return a.t[item];
-    }
-};
-
-// What the blocks of a tile share: the tensor's arrays at the tile's first element.  All of it is the same for every
-// thread, so that an access is a uniform address plus a thread's own fixed offset.
+// A tile's arrays at its first element.  All of it is the same for every thread, so that an access is a uniform
+// address plus a thread's own offset.
 template <typename W>
 struct Tile {
     W* w;
@@ -443,37 +443,54 @@ struct Tile {
 struct Constants {
     float scale, b1, omb1, b2, omb2, eps;
     f2x minus_zero;
-    uint32_t zero;
+    uint32_t zero_is_plain;
 };
 
-// One block: 8 values per lane, `cnt` of them valid (8 in a whole tile, where FULL).
-template <bool I8, bool SR, bool FULL, typename W>
-__device__ __forceinline__ void update(const Tile<W>& t, const Constants& k, const StepCoef& c, int cnt, bool vec)
+// Eight values of a lane as they are stored.
+template <bool I8, typename W> struct Loaded;
+template <typename W> struct Loaded<false, W> { float g[8], p[8], m[8], v[8]; };
+template <typename W> struct Loaded<true, W> { float g[8], p[8]; uint2 m, v; float sm, sv; };
+
+// `own`: the lane's first element in the tile; cnt of its eight are valid (8 where FULL).
+template <bool I8, bool FULL, typename W>
+__device__ __forceinline__ void load(Loaded<I8, W>& x, const Tile<W>& t, uint32_t own, int cnt, bool vec)
 {
     constexpr bool kMaster = sizeof(W) == 2;
-    const uint32_t own = threadIdx.x * 8, block = threadIdx.x / 32;
+    if constexpr (FULL) load8(t.g + own, x.g);
+    else load8(t.g + own, cnt, vec, x.g);
+    if constexpr (kMaster) load8(t.master + own, x.p);
+    else if constexpr (FULL) load8(t.w + own, x.p);
+    else load8(t.w + own, cnt, vec, x.p);
+    if constexpr (I8) {
+        x.m = *reinterpret_cast<const uint2*>(t.m + own);
+        x.v = *reinterpret_cast<const uint2*>(t.v + own);
+        x.sm = t.m_scale[own / kBlock];
+        x.sv = t.v_scale[own / kBlock];
+    } else {
+        load8(reinterpret_cast<const float*>(t.m) + own, x.m);
+        load8(reinterpret_cast<const float*>(t.v) + own, x.v);
+    }
+}
+
+// One block of 256 values, 8 per lane.
+template <bool I8, bool SR, bool FULL, typename W>
+__device__ __forceinline__ void update(const Loaded<I8, W>& in, const Tile<W>& t, const Constants& k, const StepCoef& c,
+                                       uint32_t own, int cnt, bool vec)
+{
+    constexpr bool kMaster = sizeof(W) == 2;
     const f2x nz = k.minus_zero;
     float x[8];
     f2x g[4], p[4], m[4], v[4], root[4], q[4];
-    if constexpr (FULL) load8(t.g + own, x);
-    else load8(t.g + own, cnt, vec, x);
-    pairs(x, g);
-    if constexpr (kMaster) load8(t.master + own, x);
-    else if constexpr (FULL) load8(t.w + own, x);
-    else load8(t.w + own, cnt, vec, x);
-    pairs(x, p);
+    pairs(in.g, g);
+    pairs(in.p, p);
     if constexpr (I8) {
-        const uint2 mc = *reinterpret_cast<const uint2*>(t.m + own), vc = *reinterpret_cast<const uint2*>(t.v + own);
-        decode_m(mc, t.m_scale[block], m);
-        decode_v(vc, t.v_scale[block], v);
+        decode_m(in.m, in.sm, m);
+        decode_v(in.v, in.sv, v);
     } else {
-        load8(reinterpret_cast<const float*>(t.m) + own, x);
-        pairs(x, m);
-        load8(reinterpret_cast<const float*>(t.v) + own, x);
-        pairs(x, v);
+        pairs(in.m, m);
+        pairs(in.v, v);
     }
-    // `low`, `high`: the extremes of v's bits, a zero left out where eps alone is a divisor that quotient2 takes
-    uint32_t low = 0xffffffffU, high = 0;
+    uint32_t low = 0xffffffffU, high = 0;   // the extremes of v's bits
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const f2x gj = mul2(g[j], both(k.scale));
@@ -481,23 +498,33 @@ __device__ __forceinline__ void update(const Tile<W>& t, const Constants& k, con
         v[j] = add2(term2(v[j], both(k.b2), nz), term2(mul2(gj, both(k.omb2)), gj, nz));
         float v0, v1;
         up2(v[j], v0, v1);
-        low = __viaddmin_u32(f2u(v0), k.zero, __viaddmin_u32(f2u(v1), k.zero, low));
+        low = __vimin3_u32(low, f2u(v0), f2u(v1));
         high = __vimax3_u32(high, f2u(v0), f2u(v1));
         root[j] = sqrt2(v[j]);
         q[j] = quotient2(m[j], add2(term2(root[j], both(c.inv_sqrt_bc2), nz), both(k.eps)));
     }
-    const bool plain = low < 0x0dffffffU || high >= 0x7b800000U;   // under 2^-99 or not under 2^120
-    if (__builtin_expect(plain, 0)) {
+    uint32_t zeros[2] = {0, 0};   // a 1 in the byte of each v that is 0
+    if (__builtin_expect(low < 0x0e000000U || high >= 0x7b800000U, 0)) {   // under 2^-99 or not under 2^120
+        bool ieee = !k.zero_is_plain || high >= 0x7b800000U;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            float v0, v1, m0, m1;
+            float v0, v1;
             up2(v[j], v0, v1);
-            up2(m[j], m0, m1);
-            v0 = __fsqrt_rn(v0);
-            v1 = __fsqrt_rn(v1);
-            root[j] = pk2(v0, v1);
-            q[j] = pk2(__fdiv_rn(m0, __fadd_rn(__fmul_rn(v0, c.inv_sqrt_bc2), k.eps)),
-                       __fdiv_rn(m1, __fadd_rn(__fmul_rn(v1, c.inv_sqrt_bc2), k.eps)));
+            zeros[j >> 1] |= ((f2u(v0) == 0 ? 1U : 0U) | (f2u(v1) == 0 ? 0x100U : 0U)) << (16 * (j & 1));
+            ieee |= (f2u(v0) != 0 && f2u(v0) < 0x0e000000U) || (f2u(v1) != 0 && f2u(v1) < 0x0e000000U);
+        }
+        if (ieee) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float v0, v1, m0, m1;
+                up2(v[j], v0, v1);
+                up2(m[j], m0, m1);
+                v0 = __fsqrt_rn(v0);
+                v1 = __fsqrt_rn(v1);
+                root[j] = pk2(v0, v1);
+                q[j] = pk2(__fdiv_rn(m0, __fadd_rn(__fmul_rn(v0, c.inv_sqrt_bc2), k.eps)),
+                           __fdiv_rn(m1, __fadd_rn(__fmul_rn(v1, c.inv_sqrt_bc2), k.eps)));
+            }
         }
     }
 #pragma unroll
@@ -509,6 +536,8 @@ __device__ __forceinline__ void update(const Tile<W>& t, const Constants& k, con
             m[j] = first_of(m[j], cnt - 2 * j);
             root[j] = first_of(root[j], cnt - 2 * j);
         }
+        if (cnt < 4) zeros[0] |= 0x01010101U << (8 * cnt);
+        zeros[1] |= cnt <= 4 ? 0x01010101U : cnt < 8 ? 0x01010101U << (8 * (cnt - 4)) : 0U;
     }
     singles(p, x);
     if constexpr (kMaster) store8(t.master + own, x);
@@ -525,10 +554,10 @@ __device__ __forceinline__ void update(const Tile<W>& t, const Constants& k, con
         }
         const BlockScales s = block_scales(block_max(m), block_max(root));
         *reinterpret_cast<uint2*>(t.m + own) = encode_m<SR>(m, s.to_m, r, nz);
-        *reinterpret_cast<uint2*>(t.v + own) = encode_v<SR>(root, s.to_root, r);
+        *reinterpret_cast<uint2*>(t.v + own) = encode_v<SR>(root, s.to_root, r, zeros, nz);
         if (threadIdx.x % 32 == 0) {
-            t.m_scale[block] = s.m;
-            t.v_scale[block] = s.root;
+            t.m_scale[own / kBlock] = s.m;
+            t.v_scale[own / kBlock] = s.root;
         }
     } else {
         singles(m, x);
@@ -538,37 +567,166 @@ __device__ __forceinline__ void update(const Tile<W>& t, const Constants& k, con
     }
 }
 
-// W: the weights' and gradients' type (float, or uint16_t for bf16 bits with an fp32 master).  A warp takes one block
-// of each of its CTA's tiles.
-template <bool I8, bool SR, typename W, int N>
-__global__ void __launch_bounds__(kThreads) step_kernel(const __grid_constant__ Args<N> a)
+// A CTA's way through its tiles; the same for every thread.
+template <bool I8, typename W, int N>
+struct Walk {
+    int tile, item, end;      // end: the first tile of the next tensor
+    int64_t at, left;         // the tile's first element, and the tensor's elements from there on
+    bool vec;
+
+    __device__ __forceinline__ Walk(const Args<N>& a, int first) : tile(first)
+    {
+        item = find_item(a, tile);
+        open(a);
+    }
+    __device__ __forceinline__ void open(const Args<N>& a)
+    {
+        const Item& s = a.t[item];
+        end = item + 1 < a.count ? a.t[item + 1].tile_begin : a.tiles;
+        at = (int64_t)(tile - s.tile_begin) * kTile;
+        left = s.n - at;
+        vec = s.index_vec & 1;
+    }
+    __device__ __forceinline__ bool valid(const Args<N>& a) const { return tile < a.tiles; }
+    // every block of the tile is whole and can be accessed in vectors
+    __device__ __forceinline__ bool whole() const { return vec && left >= kTile; }
+    __device__ __forceinline__ Tile<W> here(const Args<N>& a) const
+    {
+        constexpr int kMoment = I8 ? 1 : 4;   // bytes
+        const Item& s = a.t[item];
+        return Tile<W>{static_cast<W*>(s.w) + at, static_cast<const W*>(s.g) + at, s.master + at,
+                       static_cast<uint8_t*>(s.m) + at * kMoment, static_cast<uint8_t*>(s.v) + at * kMoment,
+                       s.m_scale + at / kBlock, s.v_scale + at / kBlock, (uint32_t)at};
+    }
+    __device__ __forceinline__ void next(const Args<N>& a)
+    {
+        tile += gridDim.x;
+        if (tile < end) {
+            at += (int64_t)gridDim.x * kTile;
+            left -= (int64_t)gridDim.x * kTile;
+        } else if (tile < a.tiles) {
+            do ++item; while (item + 1 < a.count && a.t[item + 1].tile_begin <= tile);
+            open(a);
+        }
+    }
+};
+
+// 8-bit moments: a warp's blocks travel through shared memory, kStages - 1 of them under way while one is computed.
+// That needs no registers for what is under way, and the copies of a warp are contiguous.
+template <typename W>
+struct Ring {
+    static constexpr int kStages = 3;
+    static constexpr int kP = 0, kG = kP + 4 * kBlock, kM = kG + (int)sizeof(W) * kBlock, kV = kM + kBlock, kS = kV + kBlock;
+    static constexpr int kBytes = kS + 16;
+};
+
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from)
 {
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(__cvta_generic_to_global(from)) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(__cvta_generic_to_global(from)), "n"(BYTES)
+                     : "memory");
+}
+
+// Start the copies of the warp's block of a tile (its first element is `b0` there).
+template <typename W>
+__device__ __forceinline__ void fetch(const Tile<W>& t, uint32_t b0, uint32_t to)
+{
+    using R = Ring<W>;
+    const uint32_t lane = threadIdx.x % 32;
+    const float* p;
+    if constexpr (sizeof(W) == 2) p = t.master;
+    else p = t.w;
+    copy_async<16>(to + R::kP + lane * 16, p + (b0 + lane * 4));
+    copy_async<16>(to + R::kP + 512 + lane * 16, p + (b0 + lane * 4) + 128);
+    constexpr int kPer = 16 / (int)sizeof(W);
+    copy_async<16>(to + R::kG + lane * 16, t.g + (b0 + lane * kPer));
+    if constexpr (sizeof(W) == 4) copy_async<16>(to + R::kG + 512 + lane * 16, t.g + (b0 + lane * kPer) + 128);
+    copy_async<8>(to + R::kM + lane * 8, t.m + (b0 + lane * 8));
+    copy_async<8>(to + R::kV + lane * 8, t.v + (b0 + lane * 8));
+    if (lane == 0) {
+        copy_async<4>(to + R::kS, t.m_scale + b0 / kBlock);
+        copy_async<4>(to + R::kS + 4, t.v_scale + b0 / kBlock);
+    }
+}
+
+__device__ __forceinline__ void shared8(const uint8_t* p, float (&x)[8])
+{
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+
+template <typename W>
+__device__ __forceinline__ void take(Loaded<true, W>& x, const uint8_t* from)
+{
+    using R = Ring<W>;
+    const uint32_t lane = threadIdx.x % 32;
+    shared8(from + R::kP + lane * 32, x.p);
+    if constexpr (sizeof(W) == 4) shared8(from + R::kG + lane * 32, x.g);
+    else load8(reinterpret_cast<const uint16_t*>(from + R::kG + lane * 16), x.g);
+    x.m = *reinterpret_cast<const uint2*>(from + R::kM + lane * 8);
+    x.v = *reinterpret_cast<const uint2*>(from + R::kV + lane * 8);
+    x.sm = *reinterpret_cast<const float*>(from + R::kS);
+    x.sv = *reinterpret_cast<const float*>(from + R::kS + 4);
+}
+
+// W: the weights' and gradients' type (float, or uint16_t for bf16 bits with an fp32 master).  A warp takes a block of
+// each of its CTA's tiles.
+template <bool I8, bool SR, typename W, int N>
+__global__ void __launch_bounds__(kThreads, kStepCtas<I8>) step_kernel(const __grid_constant__ Args<N> a)
+{
+    using R = Ring<W>;
+    __shared__ __align__(16) uint8_t ring[I8 ? kWarps * R::kStages * R::kBytes : 16];
     __shared__ bool last;
     // skip is a flag as loss scalers write it; a norm that is not finite says the same of the gradients
     if (a.skip != nullptr && !(*a.skip == 0.0f)) return;
     if (a.norm != nullptr && !(fabsf(*a.norm) <= 3.402823466e38f)) return;
-    const Constants k{a.g_scale != nullptr ? *a.g_scale : 1.0f, a.b1, a.omb1, a.b2, a.omb2, a.eps, both(a.minus_zero), a.zero};
+    const Constants k{a.g_scale != nullptr ? *a.g_scale : 1.0f, a.b1, a.omb1, a.b2, a.omb2, a.eps, both(a.minus_zero), a.zero_is_plain};
     StepCoef c;
     int current = -1;
-    Cursor<N> now(a, blockIdx.x);
-    for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
-        const Item& t = now.at(a, tile);
+    const uint32_t mine = threadIdx.x / 32 * kBlock;   // the warp's block in a tile
+    uint8_t* const slots = ring + threadIdx.x / 32 * (R::kStages * R::kBytes);
+    Walk<I8, W, N> now(a, blockIdx.x), ahead = now;
+    const auto prefetch = [&](int slot) {
+        if constexpr (I8) {
+            if (ahead.valid(a)) {
+                if (ahead.whole()) fetch(ahead.here(a), mine, (uint32_t)__cvta_generic_to_shared(slots + slot * R::kBytes));
+                ahead.next(a);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < R::kStages - 1; ++i) prefetch(i);
+    int slot = 0;
+    for (; now.valid(a); now.next(a)) {
         if (now.item != current) {
-            c = step_coef(a, t);
+            c = step_coef(a, a.t[now.item]);
             current = now.item;
         }
-        constexpr int kMoment = I8 ? 1 : 4;   // bytes
-        const int64_t at = (int64_t)(tile - t.tile_begin) * kTile, left = t.n - at;
-        const Tile<W> here{static_cast<W*>(t.w) + at, static_cast<const W*>(t.g) + at, t.master + at,
-                           static_cast<uint8_t*>(t.m) + at * kMoment, static_cast<uint8_t*>(t.v) + at * kMoment,
-                           t.m_scale + at / kBlock, t.v_scale + at / kBlock, (uint32_t)at};
-        const bool vec = t.index_vec & 1;
-        if (vec && left >= kTile) {
-            update<I8, SR, true, W>(here, k, c, 8, true);
-        } else if (threadIdx.x / 32 * kBlock < left) {
-            const int cnt = (int)(left < kTile ? left : kTile) - (int)threadIdx.x * 8;
-            update<I8, SR, false, W>(here, k, c, cnt < 0 ? 0 : cnt > 8 ? 8 : cnt, vec);
+        prefetch(slot == 0 ? R::kStages - 1 : slot - 1);
+        const uint32_t own = threadIdx.x * 8;
+        Loaded<I8, W> x;
+        if constexpr (I8) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(R::kStages - 1) : "memory");
+            __syncwarp();   // the other lanes' copies too
         }
+        const Tile<W> t = now.here(a);
+        if (now.whole()) {
+            if constexpr (I8) take(x, slots + slot * R::kBytes);
+            else load<I8, true, W>(x, t, own, 8, true);
+            update<I8, SR, true, W>(x, t, k, c, own, 8, true);
+        } else if (mine < now.left) {
+            const int64_t rest = now.left - own;
+            const int cnt = rest < 0 ? 0 : rest > 8 ? 8 : (int)rest;
+            load<I8, false, W>(x, t, own, cnt, now.vec);
+            update<I8, SR, false, W>(x, t, k, c, own, cnt, now.vec);
+        }
+        if constexpr (I8) __syncwarp();   // every lane has read this slot
+        slot = slot + 1 == R::kStages ? 0 : slot + 1;
     }
     __syncthreads();                      // this CTA has read its step counts
     if (threadIdx.x == 0) {
@@ -644,7 +802,12 @@ __global__ void __launch_bounds__(kThreads) i8_encode(const I8Args a)
         const float top = block_max(y);
         const BlockScales s = block_scales(top, top);
         uint2 c;
-        if constexpr (V) c = encode_v<false>(y, s.to_root, none);
+        if constexpr (V) {
+            uint32_t zeros[2] = {0, 0};
+#pragma unroll
+            for (int k = 0; k < 8; ++k) zeros[k >> 2] |= (x[k] > 0.0f ? 0U : 1U) << (8 * (k & 3));
+            c = encode_v<false>(y, s.to_root, none, zeros, both(a.minus_zero));
+        }
         else c = encode_m<false>(y, s.to_m, none, both(a.minus_zero));
         *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.codes) + i0) = c;
         if (lane == 0) a.scales[b] = V ? s.root : s.m;
@@ -654,6 +817,8 @@ __global__ void __launch_bounds__(kThreads) i8_encode(const I8Args a)
 // ---- host side ---------------------------------------------------------------------------------------
 
 bool off(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to != 0; }
+
+int64_t tiles_of(int64_t n) { return (n + kTile - 1) / kTile; }
 
 int check(const abx_graph_tensor& t, const abx_graph_step& h)
 {
@@ -697,27 +862,28 @@ int launch_step(const Args<N>& a, int32_t max_ctas, cudaStream_t st)
 
 // One launch for `count` tensors (indices `order`) of one dtype.
 template <int N>
-int run_batch(const abx_graph_tensor* t, const int32_t* order, int32_t count, int64_t tiles, const abx_graph_step& h,
+int run_batch(const abx_graph_tensor* t, const int32_t* order, int32_t count, const abx_graph_step& h,
               uint32_t* ticket, int32_t max_ctas, cudaStream_t st)
 {
     static thread_local Args<N> a;   // kept off the stack
     a.lr = h.lr; a.b1d = h.beta1; a.b2d = h.beta2; a.weight_decay = h.weight_decay;
     a.lr_ptr = h.lr_ptr; a.lr_f64 = h.lr_f64;
     a.g_scale = h.g_scale; a.skip = h.skip; a.norm = h.norm; a.ticket = ticket;
-    a.count = count; a.tiles = (int32_t)tiles; a.seed = h.seed;
+    a.count = count; a.seed = h.seed;
     a.b1 = (float)h.beta1; a.omb1 = (float)(1.0 - h.beta1);
     a.b2 = (float)h.beta2; a.omb2 = (float)(1.0 - h.beta2);
     a.eps = (float)h.eps;
     a.minus_zero = -0.0f;
-    a.zero = a.eps >= 0x1p-60f && a.eps <= 0x1p60f ? 0xffffffffU : 0U;
+    a.zero_is_plain = a.eps >= 0x1p-60f && a.eps <= 0x1p60f;
     int64_t next = 0;
     for (int32_t j = 0; j < count; ++j) {
         const abx_graph_tensor& s = t[order[j]];
         const uintptr_t wide = s.dtype == ABX_DT_F32 ? 32 : 16;   // bytes of 8 values
         const uint32_t vec = !off(s.w, wide) && !off(s.g, wide);
         a.t[j] = Item{s.w, s.g, s.master, s.m, s.v, s.m_scale, s.v_scale, s.step, s.n, (int32_t)next, s.index << 1 | vec};
-        next += (s.n + kTile - 1) / kTile;
+        next += tiles_of(s.n);
     }
+    a.tiles = (int32_t)next;
     const bool wide = t[order[0]].dtype == ABX_DT_F32;
     if (h.moments == ABX_DT_F32)
         return wide ? launch_step<false, false, float, N>(a, max_ctas, st) : launch_step<false, false, uint16_t, N>(a, max_ctas, st);
@@ -780,14 +946,14 @@ ABX_API int abx_graph_adamw(void* stream, const abx_graph_tensor* tensors, int32
             int64_t tiles = 0;
             for (; i < n && count < kMany; ++i) {
                 if (tensors[i].dtype != dtype || tensors[i].n == 0) continue;
-                const int64_t more = (tensors[i].n + kTile - 1) / kTile;
+                const int64_t more = tiles_of(tensors[i].n);
                 if (tiles + more > kMaxTiles) break;
                 order[count++] = i;
                 tiles += more;
             }
             if (count == 0) break;   // only other dtypes and empty tensors were left
-            const int rc = count <= kFew ? run_batch<kFew>(tensors, order, count, tiles, h, ticket, max_ctas, st)
-                                         : run_batch<kMany>(tensors, order, count, tiles, h, ticket, max_ctas, st);
+            const int rc = count <= kFew ? run_batch<kFew>(tensors, order, count, h, ticket, max_ctas, st)
+                                         : run_batch<kMany>(tensors, order, count, h, ticket, max_ctas, st);
             if (rc) return rc;
         }
     }
