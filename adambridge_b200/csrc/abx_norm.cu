@@ -51,6 +51,7 @@ struct Args {
     int32_t w_bf16;
     int32_t w_vec;      // w and b allow vector loads
     int32_t has_db;
+    int32_t kept;       // rows that a long kernel keeps in shared memory
     float eps;
 };
 
@@ -142,13 +143,13 @@ __device__ __forceinline__ void store(T* row, int64_t cols, int lane, int i, con
 
 // V values of a weight vector of either type (`fill` where there is none)
 template <bool VEC, int LANES, int V>
-__device__ __forceinline__ void load_w(const void* w, const Args& a, int lane, int i, float fill, float (&x)[V])
+__device__ __forceinline__ void load_w(const void* w, const Args& a, int64_t cols, int lane, int i, float fill, float (&x)[V])
 {
     const int64_t c0 = column<VEC, LANES, V>(lane, i, 0);
     if (w == nullptr) {
 #pragma unroll
         for (int k = 0; k < V; ++k) x[k] = fill;
-    } else if (VEC && a.w_vec && c0 < a.cols) {
+    } else if (VEC && a.w_vec && c0 < cols) {
         if (a.w_bf16) {
             const uint16_t* p = static_cast<const uint16_t*>(w) + c0;
 #pragma unroll
@@ -170,16 +171,43 @@ __device__ __forceinline__ void load_w(const void* w, const Args& a, int lane, i
         for (int k = 0; k < V; ++k) {
             const int64_t c = column<VEC, LANES, V>(lane, i, k);
             x[k] = 0.0f;
-            if (c < a.cols)
+            if (c < cols)
                 x[k] = a.w_bf16 ? u2f((uint32_t)static_cast<const uint16_t*>(w)[c] << 16) : static_cast<const float*>(w)[c];
         }
     }
 }
 
+// V weights of type W as they are stored, held by a thread for all of its rows.
+template <typename W, int V>
+struct Weights {
+    uint32_t raw[V * (int)sizeof(W) / 4];
+
+    // `fill` where there are none; 0 beyond the row
+    template <bool VEC, int LANES>
+    __device__ __forceinline__ void load(const void* w, const Args& a, int64_t cols, int lane, int i, float fill)
+    {
+        float x[V];
+        load_w<VEC, LANES, V>(w, a, cols, lane, i, fill, x);
+#pragma unroll
+        for (int k = 0; k < V * (int)sizeof(W) / 4; ++k) {
+            if constexpr (sizeof(W) == 4) raw[k] = f2u(x[k]);
+            else raw[k] = abx::pack_bf16_rne(x[2 * k], x[2 * k + 1]);   // exact: the values are bf16
+        }
+    }
+    __device__ __forceinline__ abx::f2x pair(int j) const
+    {
+        if constexpr (sizeof(W) == 4) return abx::pk2(u2f(raw[2 * j]), u2f(raw[2 * j + 1]));
+        else return abx::pk2(u2f(raw[j] << 16), u2f(raw[j] & 0xffff0000U));
+    }
+};
+
 // ---- sums over the threads that own a row -----------------------------------------------------------
 
-// K sums at once, each over LANES threads; every thread gets them.  `buf` alternates between two halves, so one
-// barrier per call is enough (a thread is at most one call ahead of another).
+// Floats of shared memory that row_sum wants: two halves of two sums per warp of the row.
+template <int LANES> __host__ __device__ constexpr int sum_floats() { return LANES > 32 ? 4 * (LANES / 32) : 1; }
+
+// K sums at once, each over the LANES threads of a row; every thread gets them.  `buf` alternates between two halves, so
+// one barrier per call is enough (a thread is at most one call ahead of another).
 template <int LANES, int K>
 __device__ __forceinline__ void row_sum(float (&s)[K], float* buf, int& half)
 {
@@ -191,15 +219,16 @@ __device__ __forceinline__ void row_sum(float (&s)[K], float* buf, int& half)
         constexpr int kW = LANES / 32;
         float* const b = buf + half * (2 * kW);
         half ^= 1;
-        if ((threadIdx.x & 31) == 0)
+        const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        if (lane == 0)
 #pragma unroll
-            for (int k = 0; k < K; ++k) b[k * kW + (threadIdx.x >> 5)] = s[k];
+            for (int k = 0; k < K; ++k) b[k * kW + warp] = s[k];
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            s[k] = (threadIdx.x & 31) < kW ? b[k * kW + (threadIdx.x & 31)] : 0.0f;
+            s[k] = lane < kW ? b[k * kW + lane] : 0.0f;
 #pragma unroll
-            for (int o = (kW < 32 ? kW : 32) / 2; o > 0; o >>= 1) s[k] += __shfl_xor_sync(0xffffffffU, s[k], o);
+            for (int o = kW / 2; o > 0; o >>= 1) s[k] += __shfl_xor_sync(0xffffffffU, s[k], o);
             if constexpr (kW < 32) s[k] = __shfl_sync(0xffffffffU, s[k], 0);
         }
     }
@@ -207,65 +236,184 @@ __device__ __forceinline__ void row_sum(float (&s)[K], float* buf, int& half)
 
 template <int LANES> __host__ __device__ constexpr int threads_of() { return LANES > 32 ? LANES : 256; }
 
+// ---- pairs: two values per FP32 instruction ------------------------------------------------------------
+
+using abx::f2x;
+using abx::fma2;
+using abx::mul2;
+using abx::pk2;
+using abx::up2;
+
+__device__ __forceinline__ f2x both(float x) { return pk2(x, x); }
+
+__device__ __forceinline__ f2x add2(f2x a, f2x b)
+{
+    f2x d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+template <int V>
+__device__ __forceinline__ void pairs(const float (&x)[V], f2x (&p)[V / 2])
+{
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) p[j] = pk2(x[2 * j], x[2 * j + 1]);
+}
+
+template <int V>
+__device__ __forceinline__ void singles(const f2x (&p)[V / 2], float (&x)[V])
+{
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) up2(p[j], x[2 * j], x[2 * j + 1]);
+}
+
+__device__ __forceinline__ float sum_of(f2x x)
+{
+    float a, b;
+    up2(x, a, b);
+    return a + b;
+}
+
+// ---- rows under way ------------------------------------------------------------------------------------
+// A thread copies its own vectors of the rows to come into shared memory and reads them back itself: no registers for
+// what is under way, and nothing to synchronize.  Vector j of stage s lies at ((s * PER + j) * threads + thread) * 16.
+
+__device__ __forceinline__ void copy_async(void* to, const void* from)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)),
+                 "l"(__cvta_generic_to_global(from)) : "memory");
+}
+
+template <int AHEAD>
+__device__ __forceinline__ void copies_but(void) { asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD) : "memory"); }
+
+__device__ __forceinline__ Raw stored(const uint8_t* p)
+{
+    const uint4 q = *reinterpret_cast<const uint4*>(p);
+    return Raw{{q.x, q.y, q.z, q.w}};
+}
+
+template <typename T, int LANES>
+__device__ __forceinline__ void start_copy(uint8_t* to, const T* row, int64_t cols, int lane, int i)
+{
+    const int64_t c = column<true, LANES, Vec<T>::V>(lane, i, 0);
+    if (c < cols) copy_async(to, row + c);
+}
+
+// Stages of 16 bytes x `vectors` per thread that fit in `bytes`, between 2 and 4.
+constexpr int stages_in(int bytes, int vectors, int threads)
+{
+    const int s = bytes / (16 * vectors * threads);
+    return s < 2 ? 2 : s > 4 ? 4 : s;
+}
+
 // ---- forward -----------------------------------------------------------------------------------------
 
-template <typename T, bool RMS, bool VEC, int LANES, int NV>
+template <bool VEC, int LANES, int NV>
+struct ForwardRing {
+    static constexpr int kThreads = threads_of<LANES>();
+    static constexpr int kStages = VEC ? stages_in(32768, NV, kThreads) : 1;
+    static constexpr int kBytes = VEC ? kStages * NV * kThreads * 16 : 16;
+};
+
+template <typename T, typename W, bool RMS, bool VEC, int LANES, int NV>
 __global__ void __launch_bounds__(threads_of<LANES>()) forward_kernel(const __grid_constant__ Args a)
 {
+    using R = ForwardRing<VEC, LANES, NV>;
     constexpr int V = Vec<T>::V, kRows = threads_of<LANES>() / LANES;
-    __shared__ float buf[LANES > 32 ? 4 * (LANES / 32) : 1];
+    __shared__ float buf[sum_floats<LANES>()];
+    __shared__ __align__(16) uint8_t ring[R::kBytes];
     int half = 0;
     const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
     const float inv = 1.0f / (float)a.cols;
-    for (int64_t row0 = (int64_t)blockIdx.x * kRows; row0 < a.rows; row0 += (int64_t)gridDim.x * kRows) {
-        const int64_t row = row0 + group;
-        const bool live = row < a.rows;          // a group without a row still takes part in the shuffles
-        const T* const x = static_cast<const T*>(a.x) + (live ? row : row0) * a.x_stride;
-        Raw raw[NV];
+    const int64_t stride = (int64_t)gridDim.x * kRows, first = (int64_t)blockIdx.x * kRows, cols = a.cols;
+    uint8_t* const mine = ring + threadIdx.x * 16;
+    const auto row_at = [&](int64_t row0) {   // a group without a row takes part with the first group's
+        return static_cast<const T*>(a.x) + (row0 + group < a.rows ? row0 + group : row0) * a.x_stride;
+    };
+    const auto prefetch = [&](int64_t row0, int stage) {
+        if constexpr (VEC) {
+            if (row0 < a.rows) {
+                const T* const x = row_at(row0);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) raw[i] = load<T, VEC, LANES>(x, a.cols, lane, i);
-        float mean = 0.0f;
-        if constexpr (!RMS) {
-            float s[1] = {0.0f};
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                float v[V];
-                unpack<T>(raw[i], v);
-#pragma unroll
-                for (int k = 0; k < V; ++k) s[0] += v[k];
+                for (int i = 0; i < NV; ++i)
+                    start_copy<T, LANES>(mine + (stage * NV + i) * (R::kThreads * 16), x, cols, lane, i);
             }
-            row_sum<LANES, 1>(s, buf, half);
-            mean = s[0] * inv;
+            asm volatile("cp.async.commit_group;" ::: "memory");
         }
-        float q[1] = {0.0f};
+    };
+    bool valid[NV];   // vectors within the row (where VEC, a vector is either wholly in it or not at all)
+    Weights<W, V> w[NV], b[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        valid[i] = column<VEC, LANES, V>(lane, i, 0) < cols;
+        w[i].template load<VEC, LANES>(a.w, a, cols, lane, i, 1.0f);
+        if constexpr (!RMS) b[i].template load<VEC, LANES>(a.b, a, cols, lane, i, 0.0f);
+    }
+#pragma unroll
+    for (int i = 0; i < R::kStages - 1; ++i) prefetch(first + i * stride, i);
+    int stage = 0;
+    for (int64_t row0 = first; row0 < a.rows; row0 += stride) {
+        prefetch(row0 + (R::kStages - 1) * stride, stage == 0 ? R::kStages - 1 : stage - 1);
+        f2x v[NV][V / 2];
+        if constexpr (VEC) copies_but<R::kStages - 1>();
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            float v[V];
-            unpack<T>(raw[i], v);
+            Raw raw = {{0U, 0U, 0U, 0U}};
+            if constexpr (!VEC) raw = load<T, VEC, LANES>(row_at(row0), cols, lane, i);
+            else if (valid[i]) raw = stored(mine + (stage * NV + i) * (R::kThreads * 16));
+            float x[V];
+            unpack<T>(raw, x);
+            pairs<V>(x, v[i]);
+        }
+        stage = stage + 1 == R::kStages ? 0 : stage + 1;
+        float mean = 0.0f;
+        if constexpr (!RMS) {
+            f2x t = 0;
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const float d = RMS || column<VEC, LANES, V>(lane, i, k) < a.cols ? v[k] - mean : 0.0f;
-                q[0] = __fmaf_rn(d, d, q[0]);
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int j = 0; j < V / 2; ++j) t = add2(t, v[i][j]);
+            float s[1] = {sum_of(t)};
+            row_sum<LANES, 1>(s, buf, half);
+            mean = s[0] * inv;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const f2x less = both(valid[i] ? -mean : 0.0f);   // what lies beyond the row stays 0
+#pragma unroll
+                for (int j = 0; j < V / 2; ++j) {
+                    v[i][j] = add2(v[i][j], less);
+                    if constexpr (!VEC) {
+                        float p, q;
+                        up2(v[i][j], p, q);
+                        v[i][j] = pk2(column<VEC, LANES, V>(lane, i, 2 * j) < cols ? p : 0.0f,
+                                      column<VEC, LANES, V>(lane, i, 2 * j + 1) < cols ? q : 0.0f);
+                    }
+                }
             }
         }
+        f2x t = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < V / 2; ++j) t = fma2(v[i][j], v[i][j], t);
+        float q[1] = {sum_of(t)};
         row_sum<LANES, 1>(q, buf, half);
         const float rstd = __frcp_rn(__fsqrt_rn(__fmaf_rn(q[0], inv, a.eps)));
-        if (!live) continue;
+        const int64_t row = row0 + group;
+        if (row >= a.rows) continue;
         T* const y = static_cast<T*>(a.y) + row * a.cols;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            float v[V], w[V], b[V];
-            unpack<T>(raw[i], v);
-            load_w<VEC, LANES, V>(a.w, a, lane, i, 1.0f, w);
-            if constexpr (RMS) {
+            float x[V];
 #pragma unroll
-                for (int k = 0; k < V; ++k) v[k] = (v[k] * rstd) * w[k];
-            } else {
-                load_w<VEC, LANES, V>(a.b, a, lane, i, 0.0f, b);
-#pragma unroll
-                for (int k = 0; k < V; ++k) v[k] = __fmaf_rn((v[k] - mean) * rstd, w[k], b[k]);
+            for (int j = 0; j < V / 2; ++j) {
+                const f2x h = mul2(v[i][j], both(rstd));
+                if constexpr (RMS) v[i][j] = mul2(h, w[i].pair(j));
+                else v[i][j] = fma2(h, w[i].pair(j), b[i].pair(j));
             }
-            store<T, VEC, LANES>(y, a.cols, lane, i, v);
+            singles<V>(v[i], x);
+            store<T, VEC, LANES>(y, cols, lane, i, x);
         }
         if (lane == 0) {
             if (!RMS && a.mean != nullptr) a.mean[row] = mean;
@@ -274,26 +422,74 @@ __global__ void __launch_bounds__(threads_of<LANES>()) forward_kernel(const __gr
     }
 }
 
-// Rows longer than a CTA's registers: three passes over the row, the later ones from the caches.
-constexpr int kLong = 1024;
+// Rows longer than a CTA's registers: three passes over the row, which is kept in shared memory where it fits and rows
+// allow vector access (each thread copies and reads its own vectors), and read again from the caches where not.
+constexpr int kLong = 512;
+
+// A thread's vector i of the row, of `count` rows of one image each (x, or x and dy).
+template <typename T, bool VEC>
+struct LongRow {
+    const Args& a;
+    uint8_t* const ring;
+    const int count;
+
+    __device__ __forceinline__ uint8_t* slot(int stage, int image, int i) const
+    {
+        return ring + ((int64_t)(stage * count + image) * a.cols * (int64_t)sizeof(T) + ((int64_t)i * kLong + threadIdx.x) * 16);
+    }
+    __device__ __forceinline__ void prefetch(const T* row, int stage, int image, int steps) const
+    {
+        for (int i = 0; i < steps; ++i)
+            if (((int64_t)i * kLong + threadIdx.x) * Vec<T>::V < a.cols)
+                copy_async(slot(stage, image, i), row + ((int64_t)i * kLong + threadIdx.x) * Vec<T>::V);
+    }
+    __device__ __forceinline__ Raw get(const T* row, int stage, int image, int i) const
+    {
+        if constexpr (VEC) {
+            if (a.kept) {
+                if (((int64_t)i * kLong + threadIdx.x) * Vec<T>::V < a.cols) return stored(slot(stage, image, i));
+                return Raw{{0U, 0U, 0U, 0U}};
+            }
+        }
+        return load<T, VEC, kLong>(row, a.cols, threadIdx.x, i);
+    }
+};
 
 template <typename T, bool RMS, bool VEC>
 __global__ void __launch_bounds__(kLong) forward_long(const __grid_constant__ Args a)
 {
     constexpr int V = Vec<T>::V;
-    __shared__ float buf[4 * (kLong / 32)];
-    int half = 0;
+    __shared__ float buf[sum_floats<kLong>()];
+    extern __shared__ __align__(16) uint8_t ring[];
+    int half = 0, stage = 0;
     const int lane = threadIdx.x;
     const float inv = 1.0f / (float)a.cols;
     const int steps = (int)((a.cols + (int64_t)kLong * V - 1) / ((int64_t)kLong * V));
+    const LongRow<T, VEC> rows{a, ring, 1};
+    const auto prefetch = [&](int64_t row, int to) {
+        if constexpr (VEC) {
+            if (a.kept && row < a.rows) rows.prefetch(static_cast<const T*>(a.x) + row * a.x_stride, to, 0, steps);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+    };
+    if (a.kept == 2) prefetch(blockIdx.x, 0);
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const T* const x = static_cast<const T*>(a.x) + row * a.x_stride;
+        if constexpr (VEC) {
+            if (a.kept == 2) {
+                prefetch(row + gridDim.x, stage ^ 1);
+                copies_but<1>();
+            } else {
+                prefetch(row, 0);
+                copies_but<0>();
+            }
+        }
         float mean = 0.0f;
         if constexpr (!RMS) {
             float s[1] = {0.0f};
             for (int i = 0; i < steps; ++i) {
                 float v[V];
-                unpack<T>(load<T, VEC, kLong>(x, a.cols, lane, i), v);
+                unpack<T>(rows.get(x, stage, 0, i), v);
 #pragma unroll
                 for (int k = 0; k < V; ++k) s[0] += v[k];
             }
@@ -303,7 +499,7 @@ __global__ void __launch_bounds__(kLong) forward_long(const __grid_constant__ Ar
         float q[1] = {0.0f};
         for (int i = 0; i < steps; ++i) {
             float v[V];
-            unpack<T>(load<T, VEC, kLong>(x, a.cols, lane, i), v);
+            unpack<T>(rows.get(x, stage, 0, i), v);
 #pragma unroll
             for (int k = 0; k < V; ++k) {
                 const float d = RMS || column<VEC, kLong, V>(lane, i, k) < a.cols ? v[k] - mean : 0.0f;
@@ -315,9 +511,9 @@ __global__ void __launch_bounds__(kLong) forward_long(const __grid_constant__ Ar
         T* const y = static_cast<T*>(a.y) + row * a.cols;
         for (int i = 0; i < steps; ++i) {
             float v[V], w[V], b[V];
-            unpack<T>(load<T, VEC, kLong>(x, a.cols, lane, i), v);
-            load_w<VEC, kLong, V>(a.w, a, lane, i, 1.0f, w);
-            load_w<VEC, kLong, V>(a.b, a, lane, i, 0.0f, b);
+            unpack<T>(rows.get(x, stage, 0, i), v);
+            load_w<VEC, kLong, V>(a.w, a, a.cols, lane, i, 1.0f, w);
+            load_w<VEC, kLong, V>(a.b, a, a.cols, lane, i, 0.0f, b);
 #pragma unroll
             for (int k = 0; k < V; ++k) v[k] = __fmaf_rn((v[k] - mean) * rstd, w[k], b[k]);
             store<T, VEC, kLong>(y, a.cols, lane, i, v);
@@ -326,112 +522,176 @@ __global__ void __launch_bounds__(kLong) forward_long(const __grid_constant__ Ar
             if (!RMS && a.mean != nullptr) a.mean[row] = mean;
             if (a.rstd != nullptr) a.rstd[row] = rstd;
         }
+        if (a.kept == 2) stage ^= 1;
     }
 }
 
 // ---- backward ----------------------------------------------------------------------------------------
 
-// dx of every row, and this CTA's part of dw and db over its rows.
-template <typename T, bool RMS, bool VEC, int LANES, int NV>
-__global__ void __launch_bounds__(threads_of<LANES>()) backward_kernel(const __grid_constant__ Args a)
+template <bool VEC, int LANES, int NV>
+struct BackwardRing {
+    static constexpr int kThreads = threads_of<LANES>();
+    static constexpr int kStages = VEC ? stages_in(65536, 2 * NV, kThreads) : 1;
+    static constexpr int kBytes = VEC ? kStages * 2 * NV * kThreads * 16 : 16;
+};
+
+// Resident CTAs of the backward kernel per SM: 1024 threads of one vector, 512 of two.
+template <int LANES, int NV>
+__host__ __device__ constexpr int backward_ctas()
 {
+    const int c = 1024 / (threads_of<LANES>() * (NV > 2 ? 4 : NV));
+    return c < 1 ? 1 : c;
+}
+
+// dx of every row, and this CTA's part of dw and db over its rows.
+template <typename T, typename W, bool RMS, bool VEC, int LANES, int NV>
+__global__ void __launch_bounds__(threads_of<LANES>(), backward_ctas<LANES, NV>()) backward_kernel(const __grid_constant__ Args a)
+{
+    using R = BackwardRing<VEC, LANES, NV>;
     constexpr int V = Vec<T>::V, kThreads = threads_of<LANES>(), kRows = kThreads / LANES;
     constexpr int kSums = RMS ? 1 : 2;
-    __shared__ float buf[LANES > 32 ? 4 * (LANES / 32) : (kThreads / 32) * LANES * NV * V];
+    __shared__ float buf[sum_floats<LANES>()];
+    extern __shared__ __align__(16) uint8_t ring[];   // the rows under way; at the end, the warps' sums
     int half = 0;
     const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
     const float inv = 1.0f / (float)a.cols;
-    float dw[NV][V], db[NV][V];
+    const int64_t stride = (int64_t)gridDim.x * kRows, first = (int64_t)blockIdx.x * kRows, cols = a.cols;
+    uint8_t* const mine = ring + threadIdx.x * 16;
+    const auto row_of = [&](int64_t row0) { return row0 + group < a.rows ? row0 + group : row0; };
+    const auto prefetch = [&](int64_t row0, int stage) {
+        if constexpr (VEC) {
+            if (row0 < a.rows) {
+                const T* const x = static_cast<const T*>(a.x) + row_of(row0) * a.x_stride;
+                const T* const dy = static_cast<const T*>(a.dy) + row_of(row0) * a.dy_stride;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int k = 0; k < V; ++k) dw[i][k] = db[i][k] = 0.0f;
-    for (int64_t row0 = (int64_t)blockIdx.x * kRows; row0 < a.rows; row0 += (int64_t)gridDim.x * kRows) {
-        const int64_t row = row0 + group;
-        const bool live = row < a.rows;
-        const T* const x = static_cast<const T*>(a.x) + (live ? row : row0) * a.x_stride;
-        const T* const dy = static_cast<const T*>(a.dy) + (live ? row : row0) * a.dy_stride;
-        Raw rx[NV], rd[NV];
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            rx[i] = load<T, VEC, LANES>(x, a.cols, lane, i);
-            rd[i] = load<T, VEC, LANES>(dy, a.cols, lane, i);
+                for (int i = 0; i < NV; ++i) {
+                    start_copy<T, LANES>(mine + (stage * 2 * NV + i) * (kThreads * 16), x, cols, lane, i);
+                    start_copy<T, LANES>(mine + (stage * 2 * NV + NV + i) * (kThreads * 16), dy, cols, lane, i);
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
         }
-        const float mean = RMS ? 0.0f : a.mean[live ? row : row0];
-        const float rstd = a.rstd[live ? row : row0];
-        float s[kSums];
+    };
+    f2x dw[NV][V / 2], db[NV][V / 2];
+    bool valid[NV];
+    Weights<W, V> w[NV];
 #pragma unroll
-        for (int k = 0; k < kSums; ++k) s[k] = 0.0f;
+    for (int i = 0; i < NV; ++i) {
+        valid[i] = column<VEC, LANES, V>(lane, i, 0) < cols;
+        w[i].template load<VEC, LANES>(a.w, a, cols, lane, i, 1.0f);
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) dw[i][j] = db[i][j] = 0;
+    }
+#pragma unroll
+    for (int i = 0; i < R::kStages - 1; ++i) prefetch(first + i * stride, i);
+    int stage = 0;
+    float next_mean = 0.0f, next_rstd = 0.0f;   // a row ahead
+    const auto statistics = [&](int64_t row0) {
+        if (row0 < a.rows) {
+            if constexpr (!RMS) next_mean = a.mean[row_of(row0)];
+            next_rstd = a.rstd[row_of(row0)];
+        }
+    };
+    statistics(first);
+    for (int64_t row0 = first; row0 < a.rows; row0 += stride) {
+        prefetch(row0 + (R::kStages - 1) * stride, stage == 0 ? R::kStages - 1 : stage - 1);
+        const int64_t row = row_of(row0);
+        const bool live = row0 + group < a.rows;
+        const float mean = next_mean, rstd = next_rstd;
+        statistics(row0 + stride);
+        if constexpr (VEC) copies_but<R::kStages - 1>();
+        f2x h[NV][V / 2], g[NV][V / 2];   // the normalized values and dy w
+        f2x s0 = 0, s1 = 0;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            float v[V], d[V], w[V];
-            unpack<T>(rx[i], v);
-            unpack<T>(rd[i], d);
-            load_w<VEC, LANES, V>(a.w, a, lane, i, 1.0f, w);
+            Raw rx = {{0U, 0U, 0U, 0U}}, rd = rx;
+            if constexpr (!VEC) {
+                rx = load<T, VEC, LANES>(static_cast<const T*>(a.x) + row * a.x_stride, cols, lane, i);
+                rd = load<T, VEC, LANES>(static_cast<const T*>(a.dy) + row * a.dy_stride, cols, lane, i);
+            } else if (valid[i]) {
+                rx = stored(mine + (stage * 2 * NV + i) * (kThreads * 16));
+                rd = stored(mine + (stage * 2 * NV + NV + i) * (kThreads * 16));
+            }
+            float x[V];
+            f2x d[V / 2];
+            unpack<T>(rx, x);
+            pairs<V>(x, h[i]);
+            unpack<T>(rd, x);
+            if (!live) {   // a group without a row adds nothing
 #pragma unroll
-            for (int k = 0; k < V; ++k) {   // beyond the row's end d is 0
-                const float h = (v[k] - mean) * rstd, t = d[k] * w[k];
-                s[0] = __fmaf_rn(t, h, s[0]);
-                if constexpr (!RMS) s[1] += t;
-                if (live) {
-                    dw[i][k] = __fmaf_rn(d[k], h, dw[i][k]);
-                    if constexpr (!RMS) db[i][k] += d[k];
+                for (int k = 0; k < V; ++k) x[k] = 0.0f;
+            }
+            pairs<V>(x, d);
+#pragma unroll
+            for (int j = 0; j < V / 2; ++j) {   // beyond the row's end d is 0
+                if constexpr (!RMS) h[i][j] = add2(h[i][j], both(-mean));
+                h[i][j] = mul2(h[i][j], both(rstd));
+                g[i][j] = mul2(d[j], w[i].pair(j));
+                s0 = fma2(g[i][j], h[i][j], s0);
+                dw[i][j] = fma2(d[j], h[i][j], dw[i][j]);
+                if constexpr (!RMS) {
+                    s1 = add2(s1, g[i][j]);
+                    db[i][j] = add2(db[i][j], d[j]);
                 }
             }
         }
+        stage = stage + 1 == R::kStages ? 0 : stage + 1;
+        float s[kSums];
+        s[0] = sum_of(s0);
+        if constexpr (!RMS) s[1] = sum_of(s1);
         row_sum<LANES, kSums>(s, buf, half);
         if (!live || a.y == nullptr) continue;
         const float c2 = s[0] * inv, c1 = RMS ? 0.0f : s[kSums - 1] * inv;
         T* const dx = static_cast<T*>(a.y) + row * a.cols;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            float v[V], d[V], w[V];
-            unpack<T>(rx[i], v);
-            unpack<T>(rd[i], d);
-            load_w<VEC, LANES, V>(a.w, a, lane, i, 1.0f, w);
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const float h = (v[k] - mean) * rstd;
-                float t = d[k] * w[k];
-                if constexpr (!RMS) t -= c1;
-                v[k] = __fmaf_rn(-h, c2, t) * rstd;
+            for (int j = 0; j < V / 2; ++j) {
+                if constexpr (!RMS) g[i][j] = add2(g[i][j], both(-c1));
+                g[i][j] = mul2(fma2(h[i][j], both(-c2), g[i][j]), both(rstd));
             }
-            store<T, VEC, LANES>(dx, a.cols, lane, i, v);
+            float x[V];
+            singles<V>(g[i], x);
+            store<T, VEC, LANES>(dx, cols, lane, i, x);
         }
     }
     if (a.partial == nullptr) return;
-    float* const out = a.partial + (int64_t)blockIdx.x * a.cols;
-    const int64_t second = (int64_t)gridDim.x * a.cols;
+    float* const out = a.partial + (int64_t)blockIdx.x * cols;
+    const int64_t second = (int64_t)gridDim.x * cols;
 #pragma unroll
     for (int which = 0; which < kSums; ++which) {
         if (which == 1 && !a.has_db) break;
+        float sums[NV][V];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) singles<V>(which ? db[i] : dw[i], sums[i]);
         if constexpr (LANES > 32) {
 #pragma unroll
             for (int i = 0; i < NV; ++i)
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
                     const int64_t c = column<VEC, LANES, V>(lane, i, k);
-                    if (c < a.cols) out[which * second + c] = which ? db[i][k] : dw[i][k];
+                    if (c < cols) out[which * second + c] = sums[i][k];
                 }
         } else {
             // the groups of a warp by shuffles, then the warps through shared memory, in order
             constexpr int kCols = LANES * NV * V;
-            __syncthreads();
+            float* const mem = reinterpret_cast<float*>(ring);
+            __syncthreads();   // every thread is through with its rows, or with the first sums
 #pragma unroll
             for (int i = 0; i < NV; ++i)
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
-                    float t = which ? db[i][k] : dw[i][k];
+                    float t = sums[i][k];
 #pragma unroll
                     for (int o = LANES; o < 32; o <<= 1) t += __shfl_xor_sync(0xffffffffU, t, o);
                     if ((threadIdx.x & 31) < LANES)
-                        buf[(threadIdx.x >> 5) * kCols + (int)column<VEC, LANES, V>(lane, i, k)] = t;
+                        mem[(threadIdx.x >> 5) * kCols + (int)column<VEC, LANES, V>(lane, i, k)] = t;
                 }
             __syncthreads();
-            for (int c = threadIdx.x; c < kCols && c < a.cols; c += kThreads) {
+            for (int c = threadIdx.x; c < kCols && c < cols; c += kThreads) {
                 float t = 0.0f;
 #pragma unroll
-                for (int j = 0; j < kThreads / 32; ++j) t += buf[j * kCols + c];
+                for (int j = 0; j < kThreads / 32; ++j) t += mem[j * kCols + c];
                 out[which * second + c] = t;
             }
         }
@@ -444,23 +704,44 @@ __global__ void __launch_bounds__(kLong) backward_long(const __grid_constant__ A
 {
     constexpr int V = Vec<T>::V;
     constexpr int kSums = RMS ? 1 : 2;
-    __shared__ float buf[4 * (kLong / 32)];
-    int half = 0;
+    __shared__ float buf[sum_floats<kLong>()];
+    extern __shared__ __align__(16) uint8_t ring[];
+    int half = 0, stage = 0;
     const int lane = threadIdx.x;
     const float inv = 1.0f / (float)a.cols;
     const int steps = (int)((a.cols + (int64_t)kLong * V - 1) / ((int64_t)kLong * V));
+    const LongRow<T, VEC> rows{a, ring, 2};
+    const auto prefetch = [&](int64_t row, int to) {
+        if constexpr (VEC) {
+            if (a.kept && row < a.rows) {
+                rows.prefetch(static_cast<const T*>(a.x) + row * a.x_stride, to, 0, steps);
+                rows.prefetch(static_cast<const T*>(a.dy) + row * a.dy_stride, to, 1, steps);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+    };
+    if (a.kept == 2) prefetch(blockIdx.x, 0);
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const T* const x = static_cast<const T*>(a.x) + row * a.x_stride;
         const T* const dy = static_cast<const T*>(a.dy) + row * a.dy_stride;
         const float mean = RMS ? 0.0f : a.mean[row], rstd = a.rstd[row];
+        if constexpr (VEC) {
+            if (a.kept == 2) {
+                prefetch(row + gridDim.x, stage ^ 1);
+                copies_but<1>();
+            } else {
+                prefetch(row, 0);
+                copies_but<0>();
+            }
+        }
         float s[kSums];
 #pragma unroll
         for (int k = 0; k < kSums; ++k) s[k] = 0.0f;
         for (int i = 0; i < steps; ++i) {
             float v[V], d[V], w[V];
-            unpack<T>(load<T, VEC, kLong>(x, a.cols, lane, i), v);
-            unpack<T>(load<T, VEC, kLong>(dy, a.cols, lane, i), d);
-            load_w<VEC, kLong, V>(a.w, a, lane, i, 1.0f, w);
+            unpack<T>(rows.get(x, stage, 0, i), v);
+            unpack<T>(rows.get(dy, stage, 1, i), d);
+            load_w<VEC, kLong, V>(a.w, a, a.cols, lane, i, 1.0f, w);
 #pragma unroll
             for (int k = 0; k < V; ++k) {
                 const float t = d[k] * w[k];
@@ -473,9 +754,9 @@ __global__ void __launch_bounds__(kLong) backward_long(const __grid_constant__ A
         T* const dx = static_cast<T*>(a.y) + row * a.cols;
         for (int i = 0; i < steps; ++i) {
             float v[V], d[V], w[V];
-            unpack<T>(load<T, VEC, kLong>(x, a.cols, lane, i), v);
-            unpack<T>(load<T, VEC, kLong>(dy, a.cols, lane, i), d);
-            load_w<VEC, kLong, V>(a.w, a, lane, i, 1.0f, w);
+            unpack<T>(rows.get(x, stage, 0, i), v);
+            unpack<T>(rows.get(dy, stage, 1, i), d);
+            load_w<VEC, kLong, V>(a.w, a, a.cols, lane, i, 1.0f, w);
 #pragma unroll
             for (int k = 0; k < V; ++k) {
                 const float h = (v[k] - mean) * rstd;
@@ -483,6 +764,7 @@ __global__ void __launch_bounds__(kLong) backward_long(const __grid_constant__ A
             }
             store<T, VEC, kLong>(dx, a.cols, lane, i, v);
         }
+        if (a.kept == 2) stage ^= 1;
     }
 }
 
@@ -529,7 +811,7 @@ __global__ void __launch_bounds__(32 * kSumRows) sums_long(const __grid_constant
     }
 }
 
-// dw (blockIdx.y 0) and db (1) from the parts: 32 columns per CTA, 8 threads per column, in a fixed order.
+// dw (blockIdx.y 0) and db (1) from the parts: 32 columns per CTA, 32 threads per column, in a fixed order.
 struct FinishArgs {
     const float* partial;
     void* out[2];
@@ -538,23 +820,26 @@ struct FinishArgs {
     int32_t bf16_out;
 };
 
-__global__ void __launch_bounds__(256) finish_sums(const __grid_constant__ FinishArgs a)
+__global__ void __launch_bounds__(1024) finish_sums(const __grid_constant__ FinishArgs a)
 {
-    __shared__ float buf[8][33];
+    __shared__ float buf[32][33];
     const int lane = threadIdx.x & 31, ty = threadIdx.x >> 5;
     const int64_t c = (int64_t)blockIdx.x * 32 + lane;
-    void* const out = blockIdx.y ? a.out[1] : a.out[0];
     const float* p = a.partial + (int64_t)blockIdx.y * a.parts * a.cols;
     float t = 0.0f;
     if (c < a.cols)
-        for (int i = ty; i < a.parts; i += 8) t += p[(int64_t)i * a.cols + c];
+#pragma unroll 8
+        for (int i = ty; i < a.parts; i += 32) t += p[(int64_t)i * a.cols + c];
     buf[ty][lane] = t;
     __syncthreads();
-    if (ty == 0 && c < a.cols) {
+    t = buf[lane][ty];   // the parts of column ty
 #pragma unroll
-        for (int j = 1; j < 8; ++j) t += buf[j][lane];
-        if (a.bf16_out) static_cast<uint16_t*>(out)[c] = (uint16_t)abx::pack_bf16_rne(t, 0.0f);
-        else static_cast<float*>(out)[c] = t;
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffU, t, o);
+    const int64_t col = (int64_t)blockIdx.x * 32 + ty;
+    if (lane == 0 && col < a.cols) {
+        void* const out = blockIdx.y ? a.out[1] : a.out[0];
+        if (a.bf16_out) static_cast<uint16_t*>(out)[col] = (uint16_t)abx::pack_bf16_rne(t, 0.0f);
+        else static_cast<float*>(out)[col] = t;
     }
 }
 
@@ -580,6 +865,16 @@ int sm_count(int* sms)
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
     return e == cudaSuccess ? ABX_OK : abx::set_error("launch geometry", e);
+}
+
+int resident(const void* kernel, int threads, size_t bytes, int* out)
+{
+    int sms = 0, per = 0;
+    if (int rc = sm_count(&sms)) return rc;
+    const cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, threads, bytes);
+    if (e != cudaSuccess) return abx::set_error("launch geometry", e);
+    *out = sms * (per > 0 ? per : 1);
+    return ABX_OK;
 }
 
 int launched(const char* what)
@@ -609,22 +904,32 @@ bool vectors(const abx_norm& n, const void* second, int64_t second_stride, const
     return n.cols % v == 0 && n.x_stride % v == 0 && second_stride % v == 0 && !off(n.x, 16) && !off(second, 16) && !off(out, 16);
 }
 
-// The shape of the row kernels: vectors per row to threads per row and vectors per thread.
-//   up to 128 vectors (1024 bf16 values): part of a warp or a warp, no barrier;  up to `most`: a CTA, two or four
-//   vectors per thread;  above: the long form.
-template <typename F>
-int by_width(int64_t nvec, int64_t most, F&& f)
+// The shape of the row kernels, by the vectors of a row: threads per row, vectors per thread.  Where rows allow vector
+// access, two vectors per thread (a row of 4096 bf16 values: 256 threads) beat one (layer norm of 16384 x 4096: 49
+// against 63 us forward, 83 against 93 backward); without it, one (20000 x 1001: 27 against 47 and 42 against 69 us).
+// Longer rows take the long kernels.  (Sharing them among a cluster of CTAs was slower: a cluster barrier per sum and
+// row, 59 us instead of 23 for 515 x 20000 forward.)
+template <bool VEC, typename F>
+int by_width(int64_t nvec, F&& f)
 {
     using std::integral_constant;
 #define ABX_ROW(L, N) return f(integral_constant<int, L>{}, integral_constant<int, N>{})
     if (nvec <= 8) ABX_ROW(8, 1);
     if (nvec <= 16) ABX_ROW(16, 1);
     if (nvec <= 32) ABX_ROW(32, 1);
-    if (nvec <= 64) ABX_ROW(32, 2);
-    if (nvec <= 128) ABX_ROW(32, 4);
-    if (nvec <= 256) ABX_ROW(128, 2);
-    if (nvec <= 512) ABX_ROW(256, 2);
-    if (nvec <= 1024 && most >= 1024) ABX_ROW(512, 2);
+    if constexpr (VEC) {
+        if (nvec <= 64) ABX_ROW(32, 2);
+        if (nvec <= 128) ABX_ROW(32, 4);
+        if (nvec <= 256) ABX_ROW(128, 2);
+        if (nvec <= 512) ABX_ROW(256, 2);
+        if (nvec <= 1024) ABX_ROW(512, 2);
+    } else {
+        if (nvec <= 64) ABX_ROW(64, 1);
+        if (nvec <= 128) ABX_ROW(128, 1);
+        if (nvec <= 256) ABX_ROW(256, 1);
+        if (nvec <= 512) ABX_ROW(512, 1);
+        if (nvec <= 1024) ABX_ROW(1024, 1);
+    }
     return f(integral_constant<int, 0>{}, integral_constant<int, 0>{});
 #undef ABX_ROW
 }
@@ -632,33 +937,63 @@ int by_width(int64_t nvec, int64_t most, F&& f)
 template <typename F>
 int by_flags(const abx_norm& n, bool vec, F&& f)
 {
-    using T = std::true_type;
+    using Y = std::true_type;
     using N = std::false_type;
-    if (n.dtype == ABX_DT_BF16) {
-        if (n.rms) return vec ? f(bf16{}, T{}, T{}) : f(bf16{}, T{}, N{});
-        return vec ? f(bf16{}, N{}, T{}) : f(bf16{}, N{}, N{});
-    }
-    if (n.rms) return vec ? f(0.0f, T{}, T{}) : f(0.0f, T{}, N{});
-    return vec ? f(0.0f, N{}, T{}) : f(0.0f, N{}, N{});
+    const auto flags = [&](auto t, auto w) {
+        if (n.rms) return vec ? f(t, w, Y{}, Y{}) : f(t, w, Y{}, N{});
+        return vec ? f(t, w, N{}, Y{}) : f(t, w, N{}, N{});
+    };
+    if (n.dtype == ABX_DT_BF16) return n.w_dtype == ABX_DT_BF16 ? flags(bf16{}, bf16{}) : flags(bf16{}, 0.0f);
+    return n.w_dtype == ABX_DT_BF16 ? flags(0.0f, bf16{}) : flags(0.0f, 0.0f);
 }
 
-constexpr int64_t kMostVectors = 1024;   // per row in the register kernels
 constexpr int kMaxGrid = 1 << 30;
 
-// CTAs of the backward pass (each has a part of the sums): two per SM, or fewer when there are few rows -- a part is
-// written and read again, 8 bytes per column, so it should cover some rows.
+// Parts of the sums: a CTA of the backward kernel each, as many as are resident, or fewer when there are few
+// rows (a part is written and read again, so it should cover some).  Long rows: row runs of sums_long, so that all column
+// tiles together fill the SMs.
+template <bool VEC>
 int backward_parts(const abx_norm& n, int sms)
 {
     const int64_t v = 16 / size_of(n.dtype), nvec = (n.cols + v - 1) / v;
-    if (nvec > kMostVectors) {   // sums_long: row runs so that all column tiles together fill the SMs
-        const int64_t tiles = (nvec + 31) / 32, want = (8 * sms + tiles - 1) / tiles, most = (n.rows + 31) / 32;
-        const int64_t p = want < most ? want : most;
-        return (int)(p > 0 ? p : 1);
+    return by_width<VEC>(nvec, [&](auto lanes, auto nv) {
+        constexpr int L = decltype(lanes)::value, NV = decltype(nv)::value;
+        if constexpr (L == 0) {
+            const int64_t tiles = (nvec + 31) / 32, want = (8 * sms + tiles - 1) / tiles, most = (n.rows + 31) / 32;
+            const int64_t p = want < most ? want : most;
+            return (int)(p > 0 ? p : 1);
+        } else {
+            constexpr int64_t rows = threads_of<L>() / L;
+            const int64_t need = (n.rows + rows - 1) / rows, all = backward_ctas<L, NV>() * (int64_t)sms;
+            return (int)(need < all ? (need > 0 ? need : 1) : all);
+        }
+    });
+}
+
+// A launch with `bytes` of dynamic shared memory; `most` CTAs, or as many as are resident.
+template <typename K>
+int launch_rows(K* kernel, int64_t most, bool all_resident, int threads, size_t bytes, const Args& a, cudaStream_t st,
+                const char* what)
+{
+    if (bytes > 49152) {
+        const cudaError_t e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        if (e != cudaSuccess) return abx::set_error(what, e);
     }
-    const int64_t rows = nvec <= 8 ? 32 : nvec <= 16 ? 16 : nvec <= 128 ? 8 : 1;   // per CTA at a time
-    const int64_t need = (n.rows + rows - 1) / rows;
-    const int64_t most = (nvec <= 256 ? 4 : 2) * (int64_t)sms;
-    return (int)(need < most ? (need > 0 ? need : 1) : most);
+    if (all_resident) {
+        int ctas = 0;
+        if (int rc = resident((const void*)kernel, threads, bytes, &ctas)) return rc;
+        if (ctas < most) most = ctas;
+    }
+    kernel<<<(unsigned)most, threads, bytes, st>>>(a);
+    return launched(what);
+}
+
+// Rows of `bytes` that a long kernel keeps in shared memory: two (the next one under way) where two CTAs then still share
+// an SM's 227 KB, one as far as it fits; 0: the row is read again instead.
+int rows_kept(int64_t bytes)
+{
+    constexpr int64_t kHalf = 110 * 1024, kAll = 220 * 1024;
+    return 2 * bytes <= kHalf ? 2 : bytes <= kAll ? 1 : 0;
 }
 
 }  // namespace
@@ -675,22 +1010,23 @@ ABX_API int abx_norm_forward(void* stream, const abx_norm* norm, void* y, float*
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     Args a = args_of(n);
     a.y = y; a.mean = mean; a.rstd = rstd;
-    return by_flags(n, vectors(n, nullptr, 0, y), [&](auto t, auto rms, auto vec) {
+    return by_flags(n, vectors(n, nullptr, 0, y), [&](auto t, auto weight, auto rms, auto vec) {
         using T = decltype(t);
+        using W = decltype(weight);
         constexpr bool kRms = decltype(rms)::value, kVec = decltype(vec)::value;
         const int64_t nvec = (n.cols + Vec<T>::V - 1) / Vec<T>::V;
-        return by_width(nvec, kMostVectors, [&](auto lanes, auto nv) {
+        return by_width<kVec>(nvec, [&](auto lanes, auto nv) {
             constexpr int L = decltype(lanes)::value, NV = decltype(nv)::value;
             if constexpr (L == 0) {
-                const int grid = (int)(n.rows < kMaxGrid ? n.rows : kMaxGrid);
-                forward_long<T, kRms, kVec><<<grid, kLong, 0, st>>>(a);
+                const int64_t bytes = n.cols * (int64_t)sizeof(T);
+                a.kept = kVec ? rows_kept(bytes) : 0;
+                return launch_rows(forward_long<T, kRms, kVec>, n.rows, true, kLong, (size_t)(a.kept * bytes), a, st,
+                                   "norm forward launch");
             } else {
                 constexpr int rows = threads_of<L>() / L;
-                const int64_t need = (n.rows + rows - 1) / rows;
-                const int grid = (int)(need < kMaxGrid ? need : kMaxGrid);
-                forward_kernel<T, kRms, kVec, L, NV><<<grid, threads_of<L>(), 0, st>>>(a);
+                return launch_rows(forward_kernel<T, W, kRms, kVec, L, NV>, (n.rows + rows - 1) / rows, true, threads_of<L>(),
+                                   0, a, st, "norm forward launch");
             }
-            return launched("norm forward launch");
         });
     });
 }
@@ -699,7 +1035,9 @@ ABX_API size_t abx_norm_backward_workspace_bytes(const abx_norm* norm)
 {
     int sms = 0;
     if (check(norm) || sm_count(&sms)) return 0;
-    return (size_t)backward_parts(*norm, sms) * (size_t)norm->cols * 4 * (norm->rms ? 1 : 2);
+    // whether the vector kernels run depends on dy and dx too: enough for either
+    const int a = backward_parts<true>(*norm, sms), b = backward_parts<false>(*norm, sms);
+    return (size_t)(a > b ? a : b) * (size_t)norm->cols * 4 * (norm->rms ? 1 : 2);
 }
 
 ABX_API int abx_norm_backward(void* stream, const abx_norm* norm, const void* dy, int64_t dy_stride, const float* mean,
@@ -716,7 +1054,8 @@ ABX_API int abx_norm_backward(void* stream, const abx_norm* norm, const void* dy
     if (!dx && !sums) return ABX_OK;
     int sms = 0;
     if (int rc = sm_count(&sms)) return rc;
-    const int parts = backward_parts(n, sms);
+    const bool vec_rows = vectors(n, dy, dy_stride, dx);
+    const int parts = vec_rows ? backward_parts<true>(n, sms) : backward_parts<false>(n, sms);
     if (sums && (!workspace || workspace_bytes < (size_t)parts * (size_t)n.cols * 4 * (n.rms ? 1 : 2))) return ABX_E_OOM;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     Args a = args_of(n);
@@ -725,17 +1064,20 @@ ABX_API int abx_norm_backward(void* stream, const abx_norm* norm, const void* dy
     a.y = dx;
     a.partial = sums ? static_cast<float*>(workspace) : nullptr;
     a.has_db = db != nullptr;
-    int rc = by_flags(n, vectors(n, dy, dy_stride, dx), [&](auto t, auto rms, auto vec) {
+    int rc = by_flags(n, vec_rows, [&](auto t, auto weight, auto rms, auto vec) {
         using T = decltype(t);
+        using W = decltype(weight);
         constexpr bool kRms = decltype(rms)::value, kVec = decltype(vec)::value;
         const int64_t nvec = (n.cols + Vec<T>::V - 1) / Vec<T>::V;
-        return by_width(nvec, kMostVectors, [&](auto lanes, auto nv) {
+        return by_width<kVec>(nvec, [&](auto lanes, auto nv) {
             constexpr int L = decltype(lanes)::value, NV = decltype(nv)::value;
             if constexpr (L == 0) {
                 if (dx && n.rows > 0) {
-                    const int grid = (int)(n.rows < kMaxGrid ? n.rows : kMaxGrid);
-                    backward_long<T, kRms, kVec><<<grid, kLong, 0, st>>>(a);
-                    if (int e = launched("norm backward launch")) return e;
+                    const int64_t bytes = 2 * n.cols * (int64_t)sizeof(T);
+                    a.kept = kVec ? rows_kept(bytes) : 0;
+                    if (int e = launch_rows(backward_long<T, kRms, kVec>, n.rows, true, kLong, (size_t)(a.kept * bytes), a, st,
+                                            "norm backward launch"))
+                        return e;
                 }
                 if (!sums) return (int)ABX_OK;
                 const int64_t tiles = (nvec + 31) / 32;
@@ -743,8 +1085,12 @@ ABX_API int abx_norm_backward(void* stream, const abx_norm* norm, const void* dy
                 sums_long<T, kRms, kVec><<<dim3((unsigned)tiles, (unsigned)parts), 32 * kSumRows, 0, st>>>(a);
                 return launched("norm sums launch");
             } else {
-                backward_kernel<T, kRms, kVec, L, NV><<<parts, threads_of<L>(), 0, st>>>(a);
-                return launched("norm backward launch");
+                using R = BackwardRing<kVec, L, NV>;
+                // the rows under way, or at the end the warps' sums
+                constexpr int sums_bytes = L > 32 ? 0 : threads_of<L>() / 32 * L * NV * Vec<T>::V * 4;
+                constexpr int bytes = R::kBytes > sums_bytes ? R::kBytes : sums_bytes;
+                return launch_rows(backward_kernel<T, W, kRms, kVec, L, NV>, parts, false, threads_of<L>(), bytes, a, st,
+                                   "norm backward launch");
             }
         });
     });
@@ -757,6 +1103,6 @@ ABX_API int abx_norm_backward(void* stream, const abx_norm* norm, const void* dy
     f.parts = parts;
     f.bf16_out = n.w_dtype == ABX_DT_BF16;
     if (!dw) f.partial += (int64_t)parts * n.cols;      // db alone
-    finish_sums<<<dim3((unsigned)((n.cols + 31) / 32), dw && db ? 2 : 1), 256, 0, st>>>(f);
+    finish_sums<<<dim3((unsigned)((n.cols + 31) / 32), dw && db ? 2 : 1), 1024, 0, st>>>(f);
     return launched("norm finish launch");
 }

@@ -41,9 +41,9 @@ def formula(x, w, b, eps, rms, dy=None):
 
 
 def depth(cols):
-    """Roundings on a value's way through a row's sum: one thread's values (at most 32 of them, or cols / 1024 in long
-    rows), then the tree."""
-    return max(32, cols / 1024) + 12
+    """Roundings on a value's way through a row's sum: one thread's values (at most 32 of them, or cols / 512 in rows
+    longer than a CTA's registers, which 512 threads share), then the tree."""
+    return max(32, cols / 512) + 12
 
 
 def check(x, w, b, eps, rms, dy=None, wants=(True, True, True)):
