@@ -309,20 +309,22 @@ constexpr int stages_in(int bytes, int vectors, int threads)
 
 // ---- forward -----------------------------------------------------------------------------------------
 
-template <bool VEC, int LANES, int NV>
+// A row of 4096 bf16 values: three stages for layer norm (90 us for 32768 rows; two: 95), two for RMS norm (92; three or
+// four: 98, its shorter kernel runs further ahead and spreads over more of the DRAM's pages).
+template <bool RMS, bool VEC, int LANES, int NV>
 struct ForwardRing {
     static constexpr int kThreads = threads_of<LANES>();
-    static constexpr int kStages = VEC ? stages_in(32768, NV, kThreads) : 1;
-    static constexpr int kBytes = VEC ? kStages * NV * kThreads * 16 : 16;
+    static constexpr int kStages = VEC ? stages_in(RMS ? 16384 : 24576, NV, kThreads) : 1;
+    static constexpr int kBytes = VEC ? kStages * NV * kThreads * 16 : 0;
 };
 
 template <typename T, typename W, bool RMS, bool VEC, int LANES, int NV>
 __global__ void __launch_bounds__(threads_of<LANES>()) forward_kernel(const __grid_constant__ Args a)
 {
-    using R = ForwardRing<VEC, LANES, NV>;
+    using R = ForwardRing<RMS, VEC, LANES, NV>;
     constexpr int V = Vec<T>::V, kRows = threads_of<LANES>() / LANES;
     __shared__ float buf[sum_floats<LANES>()];
-    __shared__ __align__(16) uint8_t ring[R::kBytes];
+    extern __shared__ __align__(16) uint8_t ring[];
     int half = 0;
     const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
     const float inv = 1.0f / (float)a.cols;
@@ -532,7 +534,7 @@ template <bool VEC, int LANES, int NV>
 struct BackwardRing {
     static constexpr int kThreads = threads_of<LANES>();
     static constexpr int kStages = VEC ? stages_in(65536, 2 * NV, kThreads) : 1;
-    static constexpr int kBytes = VEC ? kStages * 2 * NV * kThreads * 16 : 16;
+    static constexpr int kBytes = VEC ? kStages * 2 * NV * kThreads * 16 : 0;
 };
 
 // Resident CTAs of the backward kernel per SM: 1024 threads of one vector, 512 of two.
@@ -907,9 +909,10 @@ bool vectors(const abx_norm& n, const void* second, int64_t second_stride, const
 // The shape of the row kernels, by the vectors of a row: threads per row, vectors per thread.  Where rows allow vector
 // access, two vectors per thread (a row of 4096 bf16 values: 256 threads) beat one (layer norm of 16384 x 4096: 49
 // against 63 us forward, 83 against 93 backward); without it, one (20000 x 1001: 27 against 47 and 42 against 69 us).
-// Longer rows take the long kernels.  (Sharing them among a cluster of CTAs was slower: a cluster barrier per sum and
+// Forward, which has no sums to hold, a bf16 row takes three or four vectors per thread where two would need 512 threads
+// (32768 x 8192: 174 against 191 us; fp32 rows are as fast with two).  Longer rows take the long kernels.  (Sharing them among a cluster of CTAs was slower: a cluster barrier per sum and
 // row, 59 us instead of 23 for 515 x 20000 forward.)
-template <bool VEC, typename F>
+template <int V, bool VEC, bool BACKWARD, typename F>
 int by_width(int64_t nvec, F&& f)
 {
     using std::integral_constant;
@@ -922,7 +925,14 @@ int by_width(int64_t nvec, F&& f)
         if (nvec <= 128) ABX_ROW(32, 4);
         if (nvec <= 256) ABX_ROW(128, 2);
         if (nvec <= 512) ABX_ROW(256, 2);
+        if constexpr (!BACKWARD && V == 8) {
+            if (nvec <= 768) ABX_ROW(256, 3);
+            if (nvec <= 1024) ABX_ROW(256, 4);
+        }
         if (nvec <= 1024) ABX_ROW(512, 2);
+        if constexpr (!BACKWARD) {
+            if (nvec <= 2048) ABX_ROW(512, 4);
+        }
     } else {
         if (nvec <= 64) ABX_ROW(64, 1);
         if (nvec <= 128) ABX_ROW(128, 1);
@@ -956,7 +966,7 @@ template <bool VEC>
 int backward_parts(const abx_norm& n, int sms)
 {
     const int64_t v = 16 / size_of(n.dtype), nvec = (n.cols + v - 1) / v;
-    return by_width<VEC>(nvec, [&](auto lanes, auto nv) {
+    return by_width<8, VEC, true>(nvec, [&](auto lanes, auto nv) {
         constexpr int L = decltype(lanes)::value, NV = decltype(nv)::value;
         if constexpr (L == 0) {
             const int64_t tiles = (nvec + 31) / 32, want = (8 * sms + tiles - 1) / tiles, most = (n.rows + 31) / 32;
@@ -975,7 +985,7 @@ template <typename K>
 int launch_rows(K* kernel, int64_t most, bool all_resident, int threads, size_t bytes, const Args& a, cudaStream_t st,
                 const char* what)
 {
-    if (bytes > 49152) {
+    if (bytes > 40960) {   // with the kernels' static shared memory that may exceed what needs no asking
         const cudaError_t e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
         if (e != cudaSuccess) return abx::set_error(what, e);
     }
@@ -1015,7 +1025,7 @@ ABX_API int abx_norm_forward(void* stream, const abx_norm* norm, void* y, float*
         using W = decltype(weight);
         constexpr bool kRms = decltype(rms)::value, kVec = decltype(vec)::value;
         const int64_t nvec = (n.cols + Vec<T>::V - 1) / Vec<T>::V;
-        return by_width<kVec>(nvec, [&](auto lanes, auto nv) {
+        return by_width<Vec<T>::V, kVec, false>(nvec, [&](auto lanes, auto nv) {
             constexpr int L = decltype(lanes)::value, NV = decltype(nv)::value;
             if constexpr (L == 0) {
                 const int64_t bytes = n.cols * (int64_t)sizeof(T);
@@ -1025,7 +1035,7 @@ ABX_API int abx_norm_forward(void* stream, const abx_norm* norm, void* y, float*
             } else {
                 constexpr int rows = threads_of<L>() / L;
                 return launch_rows(forward_kernel<T, W, kRms, kVec, L, NV>, (n.rows + rows - 1) / rows, true, threads_of<L>(),
-                                   0, a, st, "norm forward launch");
+                                   ForwardRing<kRms, kVec, L, NV>::kBytes, a, st, "norm forward launch");
             }
         });
     });
@@ -1069,7 +1079,7 @@ ABX_API int abx_norm_backward(void* stream, const abx_norm* norm, const void* dy
         using W = decltype(weight);
         constexpr bool kRms = decltype(rms)::value, kVec = decltype(vec)::value;
         const int64_t nvec = (n.cols + Vec<T>::V - 1) / Vec<T>::V;
-        return by_width<kVec>(nvec, [&](auto lanes, auto nv) {
+        return by_width<Vec<T>::V, kVec, true>(nvec, [&](auto lanes, auto nv) {
             constexpr int L = decltype(lanes)::value, NV = decltype(nv)::value;
             if constexpr (L == 0) {
                 if (dx && n.rows > 0) {

@@ -86,7 +86,7 @@ def data(rows, cols, dtype, seed=0, offset=0.5):
     return new(rows, cols, mean=offset), new(cols, mean=1.0, std=0.2), new(cols), new(rows, cols)
 
 
-COLS = [1, 2, 7, 8, 31, 64, 65, 96, 128, 129, 256, 257, 264, 512, 1000, 1024, 1032, 2048, 2049, 4096, 4097, 8192, 8200, 11008,
+COLS = [1, 2, 7, 8, 31, 64, 65, 96, 128, 129, 256, 257, 264, 512, 1000, 1024, 1032, 2048, 2049, 4096, 4097, 8192, 8200, 11008, 12288,
         20001, 32776]
 
 
