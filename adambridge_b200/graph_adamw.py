@@ -195,7 +195,8 @@ class GraphAdamW(torch.optim.Optimizer):
     multiply-adds instead), and a gradient is scaled in fp32: the two optimizers agree to rounding, not bit for bit.
 
     A step makes the state of parameters that have none yet, which a graph cannot capture: take a step, or call
-    :meth:`prepare`, before the capture.  As with any captured backward pass, drop what holds an earlier eager graph
+    :meth:`prepare`, before the capture.  Graphs that captured steps of one optimizer update the same state: replay them
+    one after another.  As with any captured backward pass, drop what holds an earlier eager graph
     of the same parameters (its loss, its outputs) before capturing, and warm up on a side stream.
     """
 
@@ -219,6 +220,8 @@ class GraphAdamW(torch.optim.Optimizer):
             self._check_group(group)
             if not group["params"]:
                 raise ValueError("a parameter group needs at least one parameter")
+            if len({id(p) for p in group["params"]}) != len(group["params"]):
+                raise ValueError("a parameter group holds a parameter twice")
             if any(p.is_sparse for p in group["params"]):
                 raise ValueError("GraphAdamW does not support sparse parameters")
         except (ValueError, TypeError):

@@ -355,7 +355,7 @@ def train_arm(args, rank: int, world: int, local_rank: int) -> dict | None:
     import torch.nn.functional as F
     from torch.utils.checkpoint import checkpoint
 
-    from adambridge_b200 import native
+    from adambridge_b200 import native, rms_norm
     from adambridge_b200.zero import ZeroAdamBridge
 
     dev = torch.device("cuda", local_rank)
@@ -376,6 +376,8 @@ def train_arm(args, rank: int, world: int, local_rank: int) -> dict | None:
             self.weight = torch.nn.Parameter(torch.ones(hidden))
 
         def forward(self, x):
+            if args.norm == "rms_norm":
+                return rms_norm(x, self.weight, eps=1e-5)
             xf = x.float()
             return (xf * torch.rsqrt(xf.square().mean(-1, keepdim=True) + 1e-5)).to(x.dtype) * self.weight
 
@@ -481,7 +483,7 @@ def train_arm(args, rank: int, world: int, local_rank: int) -> dict | None:
             "config": {"workload": "llama-train-c5" if dims == LLAMA7B else f"llama-{dims['layers']}L-train",
                        "params": n_params, "batch_per_rank": batch, "seq_len": seq, "activation_checkpointing": True,
                        "hooks": True, "delay_updates": args.delay, "parallelism": f"zero1-dp{world}",
-                       "rounds": opt.layout.rounds,
+                       "rounds": opt.layout.rounds, "norm": args.norm,
                        "all_gather": GATHER_LABELS[opt.gather]},
             "update_kernels_ms": round(upd_ms, 3),
             "exposed_update_ms": round(exposed_ms, 3),
@@ -954,6 +956,8 @@ def main() -> int:
                     help="--workload train: delayed updates (each update overlaps the next forward)")
     ap.add_argument("--update-at-step", action="store_true",
                     help="--workload train: the hooks only reduce-scatter; every round is updated at step()")
+    ap.add_argument("--norm", default="rms_norm", choices=["rms_norm", "torch"],
+                    help="train workload: the decoder's norms on this package's kernels, or in torch operations")
     ap.add_argument("--e2e-steps", type=int, default=3)
     ap.add_argument("--cpu-seconds", type=float, default=10.0)
     ap.add_argument("--cpu-variant-seconds", type=float, default=3.0,

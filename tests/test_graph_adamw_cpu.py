@@ -41,6 +41,9 @@ def test_group_refusals_leave_no_group():
     opt = ab.GraphAdamW([torch.nn.Parameter(torch.zeros(4))])
     with pytest.raises(ValueError, match="at least one parameter"):
         opt.add_param_group({"params": []})
+    twice = torch.nn.Parameter(torch.zeros(4))
+    with pytest.raises(ValueError, match="twice"), pytest.warns(UserWarning):   # torch only warns
+        opt.add_param_group({"params": [twice, twice]})
     with pytest.raises(ValueError, match="betas"):
         opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(4))], "betas": (2.0, 0.9)})
     assert len(opt.param_groups) == 1

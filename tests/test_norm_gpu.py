@@ -288,11 +288,11 @@ class Net(torch.nn.Module):
         return ab.layer_norm(x, self.norm[2], self.bias)
 
 
-@pytest.mark.parametrize("precision", ["fp32", "int8"])
-def test_a_captured_training_step_equals_eager_ones(precision):
+@pytest.mark.parametrize("precision, width", [("fp32", 256), ("int8", 256), ("int8", 4096)])
+def test_a_captured_training_step_equals_eager_ones(precision, width):
     """Norms, their gradients, the clip and the update in one graph: five replays on new batches equal five eager steps."""
     def build():
-        net = Net(256, torch.bfloat16, 1)
+        net = Net(width, torch.bfloat16, 1)
         return net, ab.GraphAdamW(net.parameters(), lr=1e-2, precision=precision, seed=3)
 
     def step(net, opt, x, target):
@@ -304,7 +304,7 @@ def test_a_captured_training_step_equals_eager_ones(precision):
         return loss
 
     gen = torch.Generator(device="cuda").manual_seed(2)
-    batches = [[torch.empty(96, 256, dtype=torch.bfloat16, device="cuda").normal_(generator=gen) for _ in range(2)]
+    batches = [[torch.empty(96, width, dtype=torch.bfloat16, device="cuda").normal_(generator=gen) for _ in range(2)]
                for _ in range(6)]
     net, opt = build()
     eager = [float(step(net, opt, *batch)) for batch in batches]
