@@ -44,8 +44,8 @@ using abx::u2f;
 constexpr int kBlock = ABX_I8_BLOCK;      // values per scale: 8 per lane of a warp
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-// Resident CTAs per SM: at most 96 registers per thread with 8-bit moments (6 CTAs and 80 registers were as fast, 7
-// spilled: 654, 659, 725 us for 202M parameters), 64 with fp32 ones (23 against 28 us for 184 small tensors at 5).
+// Resident CTAs per SM: at most 96 registers per thread with 8-bit moments (202M parameters: 611 us; 4 CTAs 624, 6 CTAs,
+// which spill, 692), 64 with fp32 ones (184 small tensors: 18 us; 25 at 6 CTAs).
 template <bool I8> constexpr int kStepCtas = I8 ? 5 : 8;
 constexpr int kTile = kWarps * kBlock;    // elements of one tensor that a CTA takes at a time
 constexpr int kMany = 384;                // tensors per launch: the parameter block stays under 32764 bytes
@@ -416,9 +416,9 @@ __device__ __forceinline__ uint2 encode_v(const f2x (&root)[4], float f, const u
 // ---- the step ------------------------------------------------------------------------------------
 
 template <int N>
-__device__ __forceinline__ int find_item(const Args<N>& a, int tile)
+__device__ __forceinline__ int find_item(const Args<N>& a, int lo, int tile)
 {
-    int lo = 0, hi = a.count - 1;
+    int hi = a.count - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         if (a.t[mid].tile_begin <= tile) lo = mid; else hi = mid - 1;
@@ -426,10 +426,10 @@ __device__ __forceinline__ int find_item(const Args<N>& a, int tile)
     return lo;
 }
 
-// A tile's arrays at its first element.  All of it is the same for every thread, so that an access is a uniform
-// address plus a thread's own offset.
-template <typename W>
-struct Tile {
+// Where a lane's eight values lie.  A CTA's tiles of a tensor are a fixed distance apart, so the addresses are worked
+// out once per tensor and moved on from tile to tile.
+template <bool I8, typename W>
+struct Lane {
     W* w;
     const W* g;
     float* master;
@@ -437,7 +437,35 @@ struct Tile {
     uint8_t* v;
     float* m_scale;
     float* v_scale;
-    uint32_t place;   // the first element's (low 32 bits), which the rounding's random words go by
+    uint32_t place;   // of the first value in its tensor (low 32 bits), which the rounding's random words go by
+
+    __device__ __forceinline__ Lane(const Item& t, int64_t at)
+    {
+        constexpr int kMoment = I8 ? 1 : 4;   // bytes
+        at += threadIdx.x * 8;
+        w = static_cast<W*>(t.w) + at;
+        g = static_cast<const W*>(t.g) + at;
+        master = t.master + at;
+        m = static_cast<uint8_t*>(t.m) + at * kMoment;
+        v = static_cast<uint8_t*>(t.v) + at * kMoment;
+        m_scale = t.m_scale + at / kBlock;
+        v_scale = t.v_scale + at / kBlock;
+        place = (uint32_t)at;
+    }
+    __device__ __forceinline__ void advance(int64_t by)
+    {
+        constexpr int kMoment = I8 ? 1 : 4;
+        w += by;
+        if constexpr (!I8) g += by;
+        if constexpr (sizeof(W) == 2) master += by;
+        m += by * kMoment;
+        v += by * kMoment;
+        if constexpr (I8) {
+            m_scale += by / kBlock;
+            v_scale += by / kBlock;
+        }
+        place += (uint32_t)by;
+    }
 };
 
 struct Constants {
@@ -451,31 +479,31 @@ template <bool I8, typename W> struct Loaded;
 template <typename W> struct Loaded<false, W> { float g[8], p[8], m[8], v[8]; };
 template <typename W> struct Loaded<true, W> { float g[8], p[8]; uint2 m, v; float sm, sv; };
 
-// `own`: the lane's first element in the tile; cnt of its eight are valid (8 where FULL).
+// cnt of the lane's values are valid (8 where FULL).
 template <bool I8, bool FULL, typename W>
-__device__ __forceinline__ void load(Loaded<I8, W>& x, const Tile<W>& t, uint32_t own, int cnt, bool vec)
+__device__ __forceinline__ void load(Loaded<I8, W>& x, const Lane<I8, W>& t, int cnt, bool vec)
 {
     constexpr bool kMaster = sizeof(W) == 2;
-    if constexpr (FULL) load8(t.g + own, x.g);
-    else load8(t.g + own, cnt, vec, x.g);
-    if constexpr (kMaster) load8(t.master + own, x.p);
-    else if constexpr (FULL) load8(t.w + own, x.p);
-    else load8(t.w + own, cnt, vec, x.p);
+    if constexpr (FULL) load8(t.g, x.g);
+    else load8(t.g, cnt, vec, x.g);
+    if constexpr (kMaster) load8(t.master, x.p);
+    else if constexpr (FULL) load8(t.w, x.p);
+    else load8(t.w, cnt, vec, x.p);
     if constexpr (I8) {
-        x.m = *reinterpret_cast<const uint2*>(t.m + own);
-        x.v = *reinterpret_cast<const uint2*>(t.v + own);
-        x.sm = t.m_scale[own / kBlock];
-        x.sv = t.v_scale[own / kBlock];
+        x.m = *reinterpret_cast<const uint2*>(t.m);
+        x.v = *reinterpret_cast<const uint2*>(t.v);
+        x.sm = *t.m_scale;
+        x.sv = *t.v_scale;
     } else {
-        load8(reinterpret_cast<const float*>(t.m) + own, x.m);
-        load8(reinterpret_cast<const float*>(t.v) + own, x.v);
+        load8(reinterpret_cast<const float*>(t.m), x.m);
+        load8(reinterpret_cast<const float*>(t.v), x.v);
     }
 }
 
 // One block of 256 values, 8 per lane.
 template <bool I8, bool SR, bool FULL, typename W>
-__device__ __forceinline__ void update(const Loaded<I8, W>& in, const Tile<W>& t, const Constants& k, const StepCoef& c,
-                                       uint32_t own, int cnt, bool vec)
+__device__ __forceinline__ void update(const Loaded<I8, W>& in, const Lane<I8, W>& t, const Constants& k, const StepCoef& c,
+                                       int cnt, bool vec)
 {
     constexpr bool kMaster = sizeof(W) == 2;
     const f2x nz = k.minus_zero;
@@ -540,76 +568,32 @@ __device__ __forceinline__ void update(const Loaded<I8, W>& in, const Tile<W>& t
         zeros[1] |= cnt <= 4 ? 0x01010101U : cnt < 8 ? 0x01010101U << (8 * (cnt - 4)) : 0U;
     }
     singles(p, x);
-    if constexpr (kMaster) store8(t.master + own, x);
-    if constexpr (FULL) store8(t.w + own, x);
-    else store8(t.w + own, cnt, vec, x);
+    if constexpr (kMaster) store8(t.master, x);
+    if constexpr (FULL) store8(t.w, x);
+    else store8(t.w, cnt, vec, x);
     if constexpr (I8) {
         uint32_t r[8];
         if constexpr (SR) {
             uint32_t r0[4], r1[4];
-            abx::hash4(t.place + own, c.stream, r0);
-            abx::hash4(t.place + own + 4, c.stream, r1);
+            abx::hash4(t.place, c.stream, r0);
+            abx::hash4(t.place + 4, c.stream, r1);
 #pragma unroll
             for (int i = 0; i < 4; ++i) { r[i] = r0[i]; r[4 + i] = r1[i]; }
         }
         const BlockScales s = block_scales(block_max(m), block_max(root));
-        *reinterpret_cast<uint2*>(t.m + own) = encode_m<SR>(m, s.to_m, r, nz);
-        *reinterpret_cast<uint2*>(t.v + own) = encode_v<SR>(root, s.to_root, r, zeros, nz);
+        *reinterpret_cast<uint2*>(t.m) = encode_m<SR>(m, s.to_m, r, nz);
+        *reinterpret_cast<uint2*>(t.v) = encode_v<SR>(root, s.to_root, r, zeros, nz);
         if (threadIdx.x % 32 == 0) {
-            t.m_scale[own / kBlock] = s.m;
-            t.v_scale[own / kBlock] = s.root;
+            *t.m_scale = s.m;
+            *t.v_scale = s.root;
         }
     } else {
         singles(m, x);
-        store8(reinterpret_cast<float*>(t.m) + own, x);
+        store8(reinterpret_cast<float*>(t.m), x);
         singles(v, x);
-        store8(reinterpret_cast<float*>(t.v) + own, x);
+        store8(reinterpret_cast<float*>(t.v), x);
     }
 }
-
-// A CTA's way through its tiles; the same for every thread.
-template <bool I8, typename W, int N>
-struct Walk {
-    int tile, item, end;      // end: the first tile of the next tensor
-    int64_t at, left;         // the tile's first element, and the tensor's elements from there on
-    bool vec;
-
-    __device__ __forceinline__ Walk(const Args<N>& a, int first) : tile(first)
-    {
-        item = find_item(a, tile);
-        open(a);
-    }
-    __device__ __forceinline__ void open(const Args<N>& a)
-    {
-        const Item& s = a.t[item];
-        end = item + 1 < a.count ? a.t[item + 1].tile_begin : a.tiles;
-        at = (int64_t)(tile - s.tile_begin) * kTile;
-        left = s.n - at;
-        vec = s.index_vec & 1;
-    }
-    __device__ __forceinline__ bool valid(const Args<N>& a) const { return tile < a.tiles; }
-    // every block of the tile is whole and can be accessed in vectors
-    __device__ __forceinline__ bool whole() const { return vec && left >= kTile; }
-    __device__ __forceinline__ Tile<W> here(const Args<N>& a) const
-    {
-        constexpr int kMoment = I8 ? 1 : 4;   // bytes
-        const Item& s = a.t[item];
-        return Tile<W>{static_cast<W*>(s.w) + at, static_cast<const W*>(s.g) + at, s.master + at,
-                       static_cast<uint8_t*>(s.m) + at * kMoment, static_cast<uint8_t*>(s.v) + at * kMoment,
-                       s.m_scale + at / kBlock, s.v_scale + at / kBlock, (uint32_t)at};
-    }
-    __device__ __forceinline__ void next(const Args<N>& a)
-    {
-        tile += gridDim.x;
-        if (tile < end) {
-            at += (int64_t)gridDim.x * kTile;
-            left -= (int64_t)gridDim.x * kTile;
-        } else if (tile < a.tiles) {
-            do ++item; while (item + 1 < a.count && a.t[item + 1].tile_begin <= tile);
-            open(a);
-        }
-    }
-};
 
 // 8-bit moments: a warp's blocks travel through shared memory, kStages - 1 of them under way while one is computed.
 // That needs no registers for what is under way, and the copies of a warp are contiguous.
@@ -630,27 +614,53 @@ __device__ __forceinline__ void copy_async(uint32_t to, const void* from)
                      : "memory");
 }
 
-// Start the copies of the warp's block of a tile (its first element is `b0` there).
+// What a lane copies of its warp's blocks: neighbouring lanes copy neighbouring pieces.
 template <typename W>
-__device__ __forceinline__ void fetch(const Tile<W>& t, uint32_t b0, uint32_t to)
-{
-    using R = Ring<W>;
-    const uint32_t lane = threadIdx.x % 32;
+struct Fetch {
+    static constexpr int kPer = 16 / (int)sizeof(W);
     const float* p;
-    if constexpr (sizeof(W) == 2) p = t.master;
-    else p = t.w;
-    copy_async<16>(to + R::kP + lane * 16, p + (b0 + lane * 4));
-    copy_async<16>(to + R::kP + 512 + lane * 16, p + (b0 + lane * 4) + 128);
-    constexpr int kPer = 16 / (int)sizeof(W);
-    copy_async<16>(to + R::kG + lane * 16, t.g + (b0 + lane * kPer));
-    if constexpr (sizeof(W) == 4) copy_async<16>(to + R::kG + 512 + lane * 16, t.g + (b0 + lane * kPer) + 128);
-    copy_async<8>(to + R::kM + lane * 8, t.m + (b0 + lane * 8));
-    copy_async<8>(to + R::kV + lane * 8, t.v + (b0 + lane * 8));
-    if (lane == 0) {
-        copy_async<4>(to + R::kS, t.m_scale + b0 / kBlock);
-        copy_async<4>(to + R::kS + 4, t.v_scale + b0 / kBlock);
+    const W* g;
+    const uint8_t* m;
+    const uint8_t* v;
+    const float* m_scale;
+    const float* v_scale;
+
+    __device__ __forceinline__ Fetch(const Item& t, int64_t at)
+    {
+        const uint32_t lane = threadIdx.x % 32;
+        at += threadIdx.x / 32 * kBlock;
+        if constexpr (sizeof(W) == 2) p = t.master;
+        else p = static_cast<const float*>(t.w);
+        p += at + lane * 4;
+        g = static_cast<const W*>(t.g) + at + lane * kPer;
+        m = static_cast<const uint8_t*>(t.m) + at + lane * 8;
+        v = static_cast<const uint8_t*>(t.v) + at + lane * 8;
+        m_scale = t.m_scale + at / kBlock;
+        v_scale = t.v_scale + at / kBlock;
     }
-}
+    // Start the copies of this block, and move on to the next.
+    __device__ __forceinline__ void start(uint32_t to, int64_t by)
+    {
+        using R = Ring<W>;
+        const uint32_t lane = threadIdx.x % 32;
+        copy_async<16>(to + R::kP + lane * 16, p);
+        copy_async<16>(to + R::kP + 512 + lane * 16, p + 128);
+        copy_async<16>(to + R::kG + lane * 16, g);
+        if constexpr (sizeof(W) == 4) copy_async<16>(to + R::kG + 512 + lane * 16, g + 128);
+        copy_async<8>(to + R::kM + lane * 8, m);
+        copy_async<8>(to + R::kV + lane * 8, v);
+        if (lane == 0) {
+            copy_async<4>(to + R::kS, m_scale);
+            copy_async<4>(to + R::kS + 4, v_scale);
+        }
+        p += by;
+        g += by;
+        m += by;
+        v += by;
+        m_scale += by / kBlock;
+        v_scale += by / kBlock;
+    }
+};
 
 __device__ __forceinline__ void shared8(const uint8_t* p, float (&x)[8])
 {
@@ -684,49 +694,61 @@ __global__ void __launch_bounds__(kThreads, kStepCtas<I8>) step_kernel(const __g
     // skip is a flag as loss scalers write it; a norm that is not finite says the same of the gradients
     if (a.skip != nullptr && !(*a.skip == 0.0f)) return;
     if (a.norm != nullptr && !(fabsf(*a.norm) <= 3.402823466e38f)) return;
-    const Constants k{a.g_scale != nullptr ? *a.g_scale : 1.0f, a.b1, a.omb1, a.b2, a.omb2, a.eps, both(a.minus_zero), a.zero_is_plain};
-    StepCoef c;
-    int current = -1;
+    const Constants constants{a.g_scale != nullptr ? *a.g_scale : 1.0f, a.b1, a.omb1, a.b2, a.omb2, a.eps, both(a.minus_zero), a.zero_is_plain};
     const uint32_t mine = threadIdx.x / 32 * kBlock;   // the warp's block in a tile
     uint8_t* const slots = ring + threadIdx.x / 32 * (R::kStages * R::kBytes);
-    Walk<I8, W, N> now(a, blockIdx.x), ahead = now;
-    const auto prefetch = [&](int slot) {
+    const int64_t apart = (int64_t)gridDim.x * kTile;
+    int item = 0;
+    for (int tile = blockIdx.x; tile < a.tiles;) {   // from tensor to tensor
+        item = find_item(a, item, tile);
+        const Item& t = a.t[item];
+        const int end = item + 1 < a.count ? a.t[item + 1].tile_begin : a.tiles;
+        const StepCoef c = step_coef(a, t);
+        const bool vec = t.index_vec & 1;
+        int64_t at = (int64_t)(tile - t.tile_begin) * kTile;
+        Lane<I8, W> here(t, at);
+        // this CTA's whole tiles that allow vector access
+        const int64_t room = vec ? t.n - kTile - at : -1;
+        const int whole = room < 0 ? 0 : (int)(room / apart) + 1;
         if constexpr (I8) {
-            if (ahead.valid(a)) {
-                if (ahead.whole()) fetch(ahead.here(a), mine, (uint32_t)__cvta_generic_to_shared(slots + slot * R::kBytes));
-                ahead.next(a);
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        }
-    };
+            if (whole > 0) {
+                Fetch<W> ahead(t, at);
+                const auto fetch = [&](int k) {
+                    if (k < whole) ahead.start((uint32_t)__cvta_generic_to_shared(slots + k % R::kStages * R::kBytes), apart);
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                };
 #pragma unroll
-    for (int i = 0; i < R::kStages - 1; ++i) prefetch(i);
-    int slot = 0;
-    for (; now.valid(a); now.next(a)) {
-        if (now.item != current) {
-            c = step_coef(a, a.t[now.item]);
-            current = now.item;
+                for (int k = 0; k < R::kStages - 1; ++k) fetch(k);
+                for (int k = 0; k < whole; ++k) {
+                    fetch(k + R::kStages - 1);
+                    asm volatile("cp.async.wait_group %0;" ::"n"(R::kStages - 1) : "memory");
+                    __syncwarp();   // the other lanes' copies too
+                    Loaded<I8, W> x;
+                    take(x, slots + k % R::kStages * R::kBytes);
+                    update<I8, SR, true, W>(x, here, constants, c, 8, true);
+                    here.advance(apart);
+                    __syncwarp();   // every lane has read this slot
+                }
+            }
+        } else {
+            for (int k = 0; k < whole; ++k) {
+                Loaded<I8, W> x;
+                load<I8, true, W>(x, here, 8, true);
+                update<I8, SR, true, W>(x, here, constants, c, 8, true);
+                here.advance(apart);
+            }
         }
-        prefetch(slot == 0 ? R::kStages - 1 : slot - 1);
-        const uint32_t own = threadIdx.x * 8;
-        Loaded<I8, W> x;
-        if constexpr (I8) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(R::kStages - 1) : "memory");
-            __syncwarp();   // the other lanes' copies too
-        }
-        const Tile<W> t = now.here(a);
-        if (now.whole()) {
-            if constexpr (I8) take(x, slots + slot * R::kBytes);
-            else load<I8, true, W>(x, t, own, 8, true);
-            update<I8, SR, true, W>(x, t, k, c, own, 8, true);
-        } else if (mine < now.left) {
-            const int64_t rest = now.left - own;
+        tile += whole * gridDim.x;
+        at += whole * apart;
+        for (; tile < end; tile += gridDim.x, at += apart) {
+            if (at + mine >= t.n) continue;
+            const Lane<I8, W> last_lane(t, at);
+            const int64_t rest = t.n - at - (int64_t)threadIdx.x * 8;
             const int cnt = rest < 0 ? 0 : rest > 8 ? 8 : (int)rest;
-            load<I8, false, W>(x, t, own, cnt, now.vec);
-            update<I8, SR, false, W>(x, t, k, c, own, cnt, now.vec);
+            Loaded<I8, W> x;
+            load<I8, false, W>(x, last_lane, cnt, vec);
+            update<I8, SR, false, W>(x, last_lane, constants, c, cnt, vec);
         }
-        if constexpr (I8) __syncwarp();   // every lane has read this slot
-        slot = slot + 1 == R::kStages ? 0 : slot + 1;
     }
     __syncthreads();                      // this CTA has read its step counts
     if (threadIdx.x == 0) {
