@@ -910,8 +910,8 @@ bool vectors(const abx_norm& n, const void* second, int64_t second_stride, const
 // access, two vectors per thread (a row of 4096 bf16 values: 256 threads) beat one (layer norm of 16384 x 4096: 49
 // against 63 us forward, 83 against 93 backward); without it, one (20000 x 1001: 27 against 47 and 42 against 69 us).
 // Forward, which has no sums to hold, a bf16 row takes three or four vectors per thread where two would need 512 threads
-// (32768 x 8192: 174 against 191 us; fp32 rows are as fast with two).  Longer rows take the long kernels.  (Sharing them among a cluster of CTAs was slower: a cluster barrier per sum and
-// row, 59 us instead of 23 for 515 x 20000 forward.)
+// (32768 x 8192: 174 against 191 us; fp32 rows are as fast with two).  Longer rows take the long kernels.  (Sharing them
+// among a cluster of CTAs was slower: a cluster barrier per sum and row, 59 us instead of 18.5 for 515 x 20000 forward.)
 template <int V, bool VEC, bool BACKWARD, typename F>
 int by_width(int64_t nvec, F&& f)
 {

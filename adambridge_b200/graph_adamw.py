@@ -42,6 +42,10 @@ def _padded(n: int) -> int:
     return -(-n // BLOCK) * BLOCK
 
 
+def _capturing() -> bool:
+    return torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
+
+
 class StateArena:
     """The optimizer state of one parameter group: flat device buffers, parameter ``i`` at ``offsets[i]``.
 
@@ -210,7 +214,7 @@ class GraphAdamW(torch.optim.Optimizer):
         self.precision, self.stochastic, self.seed, self.max_ctas = precision, stochastic_rounding, seed, max_ctas
         self.arenas: list[StateArena] = []       # one per parameter group, once prepared
         self._native = native.load()
-        self._clip: tuple[torch.Tensor, torch.Tensor] | None = None
+        self._clip: tuple[torch.Tensor, torch.Tensor, bool] | None = None   # coefficient, norm, captured
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
     def add_param_group(self, param_group: dict[str, Any]) -> None:
@@ -248,7 +252,7 @@ class GraphAdamW(torch.optim.Optimizer):
     def prepare(self) -> "GraphAdamW":
         """Make the state (fp32 masters from the weights as they are now, zero moments) where there is none yet."""
         if len(self.arenas) < len(self.param_groups):
-            if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            if _capturing():
                 raise RuntimeError("GraphAdamW: make the state before a capture (prepare(), or an uncaptured step)")
             first = sum(len(a.params) for a in self.arenas)
             for group in self.param_groups[len(self.arenas):]:
@@ -272,7 +276,10 @@ class GraphAdamW(torch.optim.Optimizer):
         clip, self._clip = self._clip, None
         if clip is not None and grad_scale is not None:
             raise ValueError("step(grad_scale=...) after clip_grad_norm_(): the clip coefficient is the scale")
-        coef, norm = clip if clip is not None else (grad_scale, None)
+        if clip is not None and clip[2] != _capturing():
+            raise RuntimeError("clip_grad_norm_() and its step() belong into one capture, or both outside: the other's "
+                               "coefficient would be that of other gradients")
+        coef, norm = clip[:2] if clip is not None else (grad_scale, None)
         self.prepare()
         # every group is described, and so checked, before any is launched
         work = [(arena, arena.describe(), self._shared(arena, group, coef, found_inf, norm))
@@ -309,8 +316,8 @@ class GraphAdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def clip_grad_norm_(self, max_norm: float, norm_type: float = 2.0) -> torch.Tensor:
         """``torch.nn.utils.clip_grad_norm_`` over this optimizer's gradients, applied by the next :meth:`step` as it
-        reads them (see :meth:`AdamBridge.clip_grad_norm_`).  Returns the total norm; the step is skipped on the device
-        if it is not finite."""
+        reads them (see :meth:`AdamBridge.clip_grad_norm_`); both are captured, or neither.  Returns the total norm; the
+        step is skipped on the device if it is not finite."""
         if float(norm_type) != 2.0:
             raise ValueError("GraphAdamW.clip_grad_norm_ computes the L2 norm (norm_type=2) only")
         grads = [p.grad for group in self.param_groups for p in group["params"] if p.grad is not None]
@@ -328,7 +335,7 @@ class GraphAdamW(torch.optim.Optimizer):
             norms = [clip_coefficient(part, max_norm, kernels=self._native)[2] for part in parts]
             total = torch.linalg.vector_norm(torch.cat(norms))
             coef = torch.clamp(max_norm / (total + 1e-6), max=1.0).reshape(1)
-        self._clip = (coef, total.float().reshape(1))
+        self._clip = (coef, total.float().reshape(1), _capturing())
         return total
 
     # ------------------------------------------------------------------ inspection
@@ -397,7 +404,10 @@ class GraphAdamW(torch.optim.Optimizer):
                 else:
                     found.append((role, StateBuffer.from_checkpoint(saved, n, role, what)))
             step = entry["step"]
-            parsed[index] = (int(step.item() if isinstance(step, torch.Tensor) else step), master, found)
+            step = int(step.item() if isinstance(step, torch.Tensor) else step)
+            if step < 0:
+                raise ValueError(f"checkpoint parameter {index} has taken {step} steps")
+            parsed[index] = (step, master, found)
         rates = [group["lr"] for group in self.param_groups]
         super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
         for group, lr in zip(self.param_groups, rates):

@@ -370,6 +370,33 @@ def test_clip_of_mixed_gradients_is_captured():
         assert torch.equal(a, b)
 
 
+def test_a_clip_and_its_step_are_captured_together():
+    params, opt = make([300], torch.bfloat16, 6)
+    opt.prepare()
+    graph = torch.cuda.CUDAGraph()
+    opt.clip_grad_norm_(1.0)
+    with pytest.raises(RuntimeError, match="one capture"):
+        with torch.cuda.graph(graph):
+            opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.clip_grad_norm_(1.0)
+    with pytest.raises(RuntimeError, match="one capture"):
+        opt.step()
+    opt.step()                            # the clip is spent
+    assert opt.arenas[0].steps.tolist() == [1]
+
+
+def test_a_checkpoint_with_a_negative_step_is_refused():
+    _, opt = make([300], torch.bfloat16, 6)
+    opt.step()
+    saved = opt.state_dict()
+    saved["state"][0]["step"] = -1
+    with pytest.raises(ValueError, match="steps"):
+        opt.load_state_dict(saved)
+    assert opt.arenas[0].steps.tolist() == [1]
+
+
 def test_capture_needs_the_state():
     params, opt = make([300], torch.bfloat16, 6)
     graph = torch.cuda.CUDAGraph()
