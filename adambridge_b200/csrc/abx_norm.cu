@@ -574,6 +574,7 @@ __global__ void __launch_bounds__(threads_of<LANES>(), backward_ctas<LANES, NV>(
             asm volatile("cp.async.commit_group;" ::: "memory");
         }
     };
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // finish_sums may come up
     f2x dw[NV][V / 2], db[NV][V / 2];
     bool valid[NV];
     Weights<W, V> w[NV];
@@ -781,6 +782,7 @@ __global__ void __launch_bounds__(32 * kSumRows) sums_long(const __grid_constant
     const int lane = threadIdx.x & 31, ty = threadIdx.x >> 5;
     const int64_t c0 = (int64_t)blockIdx.x * kCols, left = a.cols - c0;
     const int64_t first = a.rows * blockIdx.y / gridDim.y, last = a.rows * (blockIdx.y + 1) / gridDim.y;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // finish_sums may come up
     float dw[V], db[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) dw[k] = db[k] = 0.0f;
@@ -829,6 +831,7 @@ __global__ void __launch_bounds__(1024) finish_sums(const __grid_constant__ Fini
     const int64_t c = (int64_t)blockIdx.x * 32 + lane;
     const float* p = a.partial + (int64_t)blockIdx.y * a.parts * a.cols;
     float t = 0.0f;
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // for the parts
     if (c < a.cols)
 #pragma unroll 8
         for (int i = ty; i < a.parts; i += 32) t += p[(int64_t)i * a.cols + c];
@@ -909,6 +912,8 @@ bool vectors(const abx_norm& n, const void* second, int64_t second_stride, const
 // The shape of the row kernels, by the vectors of a row: threads per row, vectors per thread.  Where rows allow vector
 // access, two vectors per thread (a row of 4096 bf16 values: 256 threads) beat one (layer norm of 16384 x 4096: 49
 // against 63 us forward, 83 against 93 backward); without it, one (20000 x 1001: 27 against 47 and 42 against 69 us).
+// So do narrow rows forward (RMS norm of 262144 x 128: 19.8 against 21.6 us); backward, which is as fast with one, keeps
+// its registers.
 // Forward, which has no sums to hold, a bf16 row takes three or four vectors per thread where two would need 512 threads
 // (32768 x 8192: 174 against 191 us; fp32 rows are as fast with two).  Longer rows take the long kernels.  (Sharing them
 // among a cluster of CTAs was slower: a cluster barrier per sum and row, 59 us instead of 18.5 for 515 x 20000 forward.)
@@ -918,6 +923,10 @@ int by_width(int64_t nvec, F&& f)
     using std::integral_constant;
 #define ABX_ROW(L, N) return f(integral_constant<int, L>{}, integral_constant<int, N>{})
     if (nvec <= 8) ABX_ROW(8, 1);
+    if constexpr (VEC && !BACKWARD) {
+        if (nvec <= 16) ABX_ROW(8, 2);
+        if (nvec <= 32) ABX_ROW(16, 2);
+    }
     if (nvec <= 16) ABX_ROW(16, 1);
     if (nvec <= 32) ABX_ROW(32, 1);
     if constexpr (VEC) {
@@ -1113,6 +1122,18 @@ ABX_API int abx_norm_backward(void* stream, const abx_norm* norm, const void* dy
     f.parts = parts;
     f.bf16_out = n.w_dtype == ABX_DT_BF16;
     if (!dw) f.partial += (int64_t)parts * n.cols;      // db alone
-    finish_sums<<<dim3((unsigned)((n.cols + 31) / 32), dw && db ? 2 : 1), 1024, 0, st>>>(f);
+    // Brought up while the parts are being computed, it waits for them on the device: 25.6 against 26.8 us for the backward
+    // pass of 4096 x 4096.
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t shape = {};
+    shape.gridDim = dim3((unsigned)((n.cols + 31) / 32), dw && db ? 2 : 1);
+    shape.blockDim = dim3(1024);
+    shape.stream = st;
+    shape.attrs = &early;
+    shape.numAttrs = 1;
+    if (const cudaError_t e = cudaLaunchKernelEx(&shape, finish_sums, f); e != cudaSuccess)
+        return abx::set_error("norm finish launch", e);
     return launched("norm finish launch");
 }
