@@ -228,7 +228,8 @@ __device__ __forceinline__ void row_sum(float (&s)[K], float* buf, int& half)
         for (int k = 0; k < K; ++k) {
             s[k] = lane < kW ? b[k * kW + lane] : 0.0f;
 #pragma unroll
-            for (int o = kW / 2; o > 0; o >>= 1) s[k] += __shfl_xor_sync(0xffffffffU, s[k], o);
+            for (int o = kW > 16 ? 16 : kW > 8 ? 8 : kW > 4 ? 4 : kW > 2 ? 2 : 1; o > 0; o >>= 1)
+                s[k] += __shfl_xor_sync(0xffffffffU, s[k], o);
             if constexpr (kW < 32) s[k] = __shfl_sync(0xffffffffU, s[k], 0);
         }
     }
@@ -293,6 +294,36 @@ __device__ __forceinline__ Raw stored(const uint8_t* p)
     return Raw{{q.x, q.y, q.z, q.w}};
 }
 
+// Where rows do not allow that, a thread loads the values of its next row into registers while it computes one (8000 x 4097
+// in bf16: 67 instead of 113 us forward, on 512 threads); forward not where a row is a warp's or less and other warps hide
+// the wait (300000 x 37 in fp32: 20 instead of 25 us).
+template <typename T, int LANES, int NV>
+struct Ahead {
+    static constexpr int V = Vec<T>::V;
+    uint32_t e[NV][V];
+
+    __device__ __forceinline__ void load(const T* row, int64_t cols, int lane)
+    {
+        const T* const p = row + lane;
+        const int left = (int)cols - lane;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                e[i][k] = 0U;
+                if ((i * V + k) * LANES < left) {
+                    if constexpr (V == 8) e[i][k] = p[(i * V + k) * LANES].bits;
+                    else e[i][k] = f2u(p[(i * V + k) * LANES]);
+                }
+            }
+    }
+    __device__ __forceinline__ void values(int i, float (&x)[V]) const
+    {
+#pragma unroll
+        for (int k = 0; k < V; ++k) x[k] = u2f(V == 8 ? e[i][k] << 16 : e[i][k]);
+    }
+};
+
 template <typename T, int LANES>
 __device__ __forceinline__ void start_copy(uint8_t* to, const T* row, int64_t cols, int lane, int i)
 {
@@ -355,19 +386,27 @@ __global__ void __launch_bounds__(threads_of<LANES>()) forward_kernel(const __gr
 #pragma unroll
     for (int i = 0; i < R::kStages - 1; ++i) prefetch(first + i * stride, i);
     int stage = 0;
+    constexpr bool kEarly = !VEC && LANES * NV > 32;
+    Ahead<T, LANES, NV> ahead;
+    if constexpr (kEarly) if (first < a.rows) ahead.load(row_at(first), cols, lane);
     for (int64_t row0 = first; row0 < a.rows; row0 += stride) {
         prefetch(row0 + (R::kStages - 1) * stride, stage == 0 ? R::kStages - 1 : stage - 1);
         f2x v[NV][V / 2];
         if constexpr (VEC) copies_but<R::kStages - 1>();
+        else if constexpr (!kEarly) ahead.load(row_at(row0), cols, lane);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            Raw raw = {{0U, 0U, 0U, 0U}};
-            if constexpr (!VEC) raw = load<T, VEC, LANES>(row_at(row0), cols, lane, i);
-            else if (valid[i]) raw = stored(mine + (stage * NV + i) * (R::kThreads * 16));
             float x[V];
-            unpack<T>(raw, x);
+            if constexpr (VEC) {
+                Raw raw = {{0U, 0U, 0U, 0U}};
+                if (valid[i]) raw = stored(mine + (stage * NV + i) * (R::kThreads * 16));
+                unpack<T>(raw, x);
+            } else {
+                ahead.values(i, x);
+            }
             pairs<V>(x, v[i]);
         }
+        if constexpr (kEarly) if (row0 + stride < a.rows) ahead.load(row_at(row0 + stride), cols, lane);
         stage = stage + 1 == R::kStages ? 0 : stage + 1;
         float mean = 0.0f;
         if constexpr (!RMS) {
@@ -537,17 +576,18 @@ struct BackwardRing {
     static constexpr int kBytes = VEC ? kStages * 2 * NV * kThreads * 16 : 0;
 };
 
-// Resident CTAs of the backward kernel per SM: 1024 threads of one vector, 512 of two.
-template <int LANES, int NV>
+// Resident CTAs of the backward kernel per SM: 1024 threads of one vector, 512 of two; 768 of one where values are accessed
+// one by one and a row ahead takes registers.
+template <bool VEC, int LANES, int NV>
 __host__ __device__ constexpr int backward_ctas()
 {
-    const int c = 1024 / (threads_of<LANES>() * (NV > 2 ? 4 : NV));
+    const int c = VEC ? 1024 / (threads_of<LANES>() * (NV > 2 ? 4 : NV)) : (NV == 1 ? 768 : 512) / threads_of<LANES>();
     return c < 1 ? 1 : c;
 }
 
 // dx of every row, and this CTA's part of dw and db over its rows.
 template <typename T, typename W, bool RMS, bool VEC, int LANES, int NV>
-__global__ void __launch_bounds__(threads_of<LANES>(), backward_ctas<LANES, NV>()) backward_kernel(const __grid_constant__ Args a)
+__global__ void __launch_bounds__(threads_of<LANES>(), backward_ctas<VEC, LANES, NV>()) backward_kernel(const __grid_constant__ Args a)
 {
     using R = BackwardRing<VEC, LANES, NV>;
     constexpr int V = Vec<T>::V, kThreads = threads_of<LANES>(), kRows = kThreads / LANES;
@@ -596,6 +636,14 @@ __global__ void __launch_bounds__(threads_of<LANES>(), backward_ctas<LANES, NV>(
         }
     };
     statistics(first);
+    Ahead<T, LANES, NV> next_x, next_dy;
+    const auto look_ahead = [&](int64_t row0) {
+        if (row0 >= a.rows) return;
+        next_x.load(static_cast<const T*>(a.x) + row_of(row0) * a.x_stride, cols, lane);
+        next_dy.load(static_cast<const T*>(a.dy) + row_of(row0) * a.dy_stride, cols, lane);
+    };
+    constexpr bool kEarly = !VEC && NV < 3;   // three vectors have no registers for it
+    if constexpr (kEarly) look_ahead(first);
     for (int64_t row0 = first; row0 < a.rows; row0 += stride) {
         prefetch(row0 + (R::kStages - 1) * stride, stage == 0 ? R::kStages - 1 : stage - 1);
         const int64_t row = row_of(row0);
@@ -603,23 +651,26 @@ __global__ void __launch_bounds__(threads_of<LANES>(), backward_ctas<LANES, NV>(
         const float mean = next_mean, rstd = next_rstd;
         statistics(row0 + stride);
         if constexpr (VEC) copies_but<R::kStages - 1>();
+        else if constexpr (!kEarly) look_ahead(row0);
         f2x h[NV][V / 2], g[NV][V / 2];   // the normalized values and dy w
         f2x s0 = 0, s1 = 0;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            Raw rx = {{0U, 0U, 0U, 0U}}, rd = rx;
-            if constexpr (!VEC) {
-                rx = load<T, VEC, LANES>(static_cast<const T*>(a.x) + row * a.x_stride, cols, lane, i);
-                rd = load<T, VEC, LANES>(static_cast<const T*>(a.dy) + row * a.dy_stride, cols, lane, i);
-            } else if (valid[i]) {
-                rx = stored(mine + (stage * 2 * NV + i) * (kThreads * 16));
-                rd = stored(mine + (stage * 2 * NV + NV + i) * (kThreads * 16));
-            }
-            float x[V];
+            float x[V], y[V];
             f2x d[V / 2];
-            unpack<T>(rx, x);
-            pairs<V>(x, h[i]);
-            unpack<T>(rd, x);
+            if constexpr (VEC) {
+                Raw rx = {{0U, 0U, 0U, 0U}}, rd = rx;
+                if (valid[i]) {
+                    rx = stored(mine + (stage * 2 * NV + i) * (kThreads * 16));
+                    rd = stored(mine + (stage * 2 * NV + NV + i) * (kThreads * 16));
+                }
+                unpack<T>(rx, y);
+                unpack<T>(rd, x);
+            } else {
+                next_x.values(i, y);
+                next_dy.values(i, x);
+            }
+            pairs<V>(y, h[i]);
             if (!live) {   // a group without a row adds nothing
 #pragma unroll
                 for (int k = 0; k < V; ++k) x[k] = 0.0f;
@@ -638,6 +689,7 @@ __global__ void __launch_bounds__(threads_of<LANES>(), backward_ctas<LANES, NV>(
                 }
             }
         }
+        if constexpr (kEarly) look_ahead(row0 + stride);
         stage = stage + 1 == R::kStages ? 0 : stage + 1;
         float s[kSums];
         s[0] = sum_of(s0);
@@ -909,14 +961,18 @@ bool vectors(const abx_norm& n, const void* second, int64_t second_stride, const
     return n.cols % v == 0 && n.x_stride % v == 0 && second_stride % v == 0 && !off(n.x, 16) && !off(second, 16) && !off(out, 16);
 }
 
-// The shape of the row kernels, by the vectors of a row: threads per row, vectors per thread.  Where rows allow vector
-// access, two vectors per thread (a row of 4096 bf16 values: 256 threads) beat one (layer norm of 16384 x 4096: 49
-// against 63 us forward, 83 against 93 backward); without it, one (20000 x 1001: 27 against 47 and 42 against 69 us).
-// So do narrow rows forward (RMS norm of 262144 x 128: 19.8 against 21.6 us); backward, which is as fast with one, keeps
-// its registers.
-// Forward, which has no sums to hold, a bf16 row takes three or four vectors per thread where two would need 512 threads
-// (32768 x 8192: 174 against 191 us; fp32 rows are as fast with two).  Longer rows take the long kernels.  (Sharing them
-// among a cluster of CTAs was slower: a cluster barrier per sum and row, 59 us instead of 18.5 for 515 x 20000 forward.)
+// The shape of the row kernels, by the vectors of a row: threads per row, vectors per thread.  Two vectors per thread (a
+// row of 4096 bf16 values: 256 threads) beat one (layer norm of 16384 x 4096: 49 against 63 us forward, 83 against 93
+// backward), narrow rows forward too (RMS norm of 262144 x 128: 19.8 against 21.6 us); backward these, as fast with one,
+// keep their registers.  Forward, which has no sums to hold, a bf16 row takes three or four vectors per thread where two
+// would need 512 threads (32768 x 8192: 174 against 191 us; fp32 rows are as fast with two).  Three vectors with sums spill
+// a few registers, which still beats the long kernels' second pass over x and dy (8192 x 12288 backward: 156 against 245 us;
+// 5000 x 10001: 142 against 197).
+// Where values are accessed one by one, instructions count, and so do threads without a value: finer steps (8000 x 4097 in
+// bf16: 51 and 70 us against 67 and 95 with 512 threads; 100000 x 301: 39 and 58 against 44 and 57 with 64 vectors' room,
+// 54 and 81 with one vector per thread).
+// Longer rows take the long kernels.  (Sharing them among a cluster of CTAs was slower: a cluster barrier per sum and row,
+// 59 us instead of 18.5 for 515 x 20000 forward.)
 template <int V, bool VEC, bool BACKWARD, typename F>
 int by_width(int64_t nvec, F&& f)
 {
@@ -926,9 +982,10 @@ int by_width(int64_t nvec, F&& f)
     if constexpr (VEC && !BACKWARD) {
         if (nvec <= 16) ABX_ROW(8, 2);
         if (nvec <= 32) ABX_ROW(16, 2);
+    } else {
+        if (nvec <= 16) ABX_ROW(16, 1);
+        if (nvec <= 32) ABX_ROW(32, 1);
     }
-    if (nvec <= 16) ABX_ROW(16, 1);
-    if (nvec <= 32) ABX_ROW(32, 1);
     if constexpr (VEC) {
         if (nvec <= 64) ABX_ROW(32, 2);
         if (nvec <= 128) ABX_ROW(32, 4);
@@ -939,15 +996,32 @@ int by_width(int64_t nvec, F&& f)
             if (nvec <= 1024) ABX_ROW(256, 4);
         }
         if (nvec <= 1024) ABX_ROW(512, 2);
-        if constexpr (!BACKWARD) {
-            if (nvec <= 2048) ABX_ROW(512, 4);
-        }
+        if (nvec <= 1536) ABX_ROW(512, 3);
+    } else if constexpr (!BACKWARD) {
+        if (nvec <= 48) ABX_ROW(16, 3);
+        if (nvec <= 64) ABX_ROW(32, 2);
+        if (nvec <= 96) ABX_ROW(32, 3);
+        if (nvec <= 128) ABX_ROW(64, 2);
+        if (nvec <= 192) ABX_ROW(64, 3);
+        if (nvec <= 256) ABX_ROW(128, 2);
+        if (nvec <= 384) ABX_ROW(128, 3);
+        if (nvec <= 512) ABX_ROW(256, 2);
+        if (nvec <= 768) ABX_ROW(256, 3);
+        if (nvec <= 1024) ABX_ROW(512, 2);
+        if (nvec <= 1536) ABX_ROW(512, 3);
     } else {
-        if (nvec <= 64) ABX_ROW(64, 1);
-        if (nvec <= 128) ABX_ROW(128, 1);
-        if (nvec <= 256) ABX_ROW(256, 1);
-        if (nvec <= 512) ABX_ROW(512, 1);
-        if (nvec <= 1024) ABX_ROW(1024, 1);
+        if (nvec <= 64) ABX_ROW(32, 2);
+        if (nvec <= 128) ABX_ROW(64, 2);
+        if (nvec <= 192) ABX_ROW(96, 2);
+        if (nvec <= 256) ABX_ROW(128, 2);
+        if (nvec <= 384) ABX_ROW(192, 2);
+        if (nvec <= 512) ABX_ROW(256, 2);
+        if (nvec <= 768) ABX_ROW(384, 2);
+        if (nvec <= 1024) ABX_ROW(512, 2);
+        if (nvec <= 1536) ABX_ROW(512, 3);
+    }
+    if constexpr (!BACKWARD) {
+        if (nvec <= 2048) ABX_ROW(512, 4);
     }
     return f(integral_constant<int, 0>{}, integral_constant<int, 0>{});
 #undef ABX_ROW
@@ -983,7 +1057,7 @@ int backward_parts(const abx_norm& n, int sms)
             return (int)(p > 0 ? p : 1);
         } else {
             constexpr int64_t rows = threads_of<L>() / L;
-            const int64_t need = (n.rows + rows - 1) / rows, all = backward_ctas<L, NV>() * (int64_t)sms;
+            const int64_t need = (n.rows + rows - 1) / rows, all = backward_ctas<VEC, L, NV>() * (int64_t)sms;
             return (int)(need < all ? (need > 0 ? need : 1) : all);
         }
     });

@@ -3,12 +3,14 @@ kernels; strides, types, empty and special rows, differences, determinism, strea
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import pytest
 import torch
 
 import adambridge_b200 as ab
+from adambridge_b200 import native
 
 pytestmark = pytest.mark.gpu
 
@@ -148,6 +150,52 @@ def test_strides(cols, dtype):
     check(wide[:, :cols].contiguous(), odd, odd.clone(), 1e-5, False, wide[:, :cols])
     check(wide[0, :cols].detach(), w, b, 1e-5, False, wide[1, :cols])          # one axis
     assert torch.equal(wide, keep)
+
+
+@pytest.mark.parametrize("cols", [1, 3, 9, 33, 61, 121, 129, 250, 505, 1001, 2050, 4097, 5121, 8185, 9001, 17001, 20003])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_between_other_data(dtype, cols):
+    """Rows that start and end anywhere in their 16 bytes, alike in all tensors or not, through the C entry points: NaNs
+    before the first row, behind the last and between padded ones stay out of the result, and so does the result of them.
+    Bounds as in `check`."""
+    kernels = native.load()
+    lib, e = kernels._lib, 5e-6
+    rows = 3000 if cols < 130 else 300 if cols < 6000 else 150     # more than the CTAs that are resident take at once
+    n, half = depth(cols), OUT[dtype]
+    _, w, b, _ = data(1, cols, dtype, cols)
+    for at, pad, out_at in ((0, 0, 0), (1, 0, 1), (3, 8, 3), (5, 0, 2), (0, 3, 0)):
+        stride, room = cols + pad, 16
+        def place(seed, start, gap):
+            gen = torch.Generator(device="cuda").manual_seed(seed)
+            buf = torch.full((room + start + rows * (cols + gap) + room,), float("nan"), dtype=dtype, device="cuda")
+            view = torch.as_strided(buf, (rows, cols), (cols + gap, 1), room + start)
+            view.normal_(0.5, 1.0, generator=gen)
+            return buf, view
+        _, x = place(1, at, pad)
+        _, dy = place(2, out_at, 0)
+        (ybuf, y), (dxbuf, dx) = place(3, out_at, 0), place(4, out_at, 0)
+        stats = torch.empty(2, rows, device="cuda")
+        spec = native.Norm(x=x.data_ptr(), w=w.data_ptr(), b=b.data_ptr(), rows=rows, cols=cols, x_stride=stride,
+                           dtype=native.dtype_code_of(dtype), w_dtype=native.dtype_code_of(dtype), rms=0, eps=e)
+        stream = torch.cuda.current_stream().cuda_stream
+        p = ctypes.byref(spec)
+        assert lib.abx_norm_forward(stream, p, y.data_ptr(), stats[0].data_ptr(), stats[1].data_ptr()) == 0
+        size = lib.abx_norm_backward_workspace_bytes(p)
+        ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+        dw, db = torch.empty_like(w), torch.empty_like(b)
+        assert lib.abx_norm_backward(stream, p, dy.data_ptr(), cols, stats[0].data_ptr(), stats[1].data_ptr(), dx.data_ptr(),
+                                     dw.data_ptr(), db.data_ptr(), ws.data_ptr(), size) == 0
+        want = formula(x, w, b, spec.eps, False, dy)
+        wa, m = w.double().abs(), rows / 100 + 64
+        bounds = {"y": (y, (2 * n + 8) * E * want["h_size"] * wa + 2 * E * (want["y"].abs() + b.double().abs())),
+                  "dx": (dx, (4 * n + 16) * E * want["dx_size"]), "dw": (dw, (2 * n + 8 + m) * E * want["dw_size"]),
+                  "db": (db, (2 * n + 8 + m) * E * want["db_size"])}
+        for name, (got, bound) in bounds.items():
+            off = (got.double() - want[name]).abs()
+            assert bool((off <= bound + half * want[name].abs() * (1 + 1e-3) + 1e-37).all()), (name, at, pad, float(off.max()))
+        for buf, view in ((ybuf, y), (dxbuf, dx)):
+            view.fill_(float("nan"))
+            assert bool(buf.isnan().all())
 
 
 def test_no_rows():
