@@ -463,7 +463,7 @@ __global__ void __launch_bounds__(threads_of<LANES>()) forward_kernel(const __gr
     }
 }
 
-// Rows longer than a CTA's registers: three passes over the row, which is kept in shared memory where it fits and rows
+// Rows longer than a CTA's registers (more than 2560 vectors): three passes over the row, which is kept in shared memory where it fits and rows
 // allow vector access (each thread copies and reads its own vectors), and read again from the caches where not.
 constexpr int kLong = 512;
 
@@ -576,12 +576,17 @@ struct BackwardRing {
     static constexpr int kBytes = VEC ? kStages * 2 * NV * kThreads * 16 : 0;
 };
 
+// With three vectors or more per thread the sums leave no registers for a row: it is read from shared memory twice.
+template <bool VEC, int LANES, int NV>
+__host__ __device__ constexpr bool twice() { return VEC && LANES > 32 && NV > 2; }
+
 // Resident CTAs of the backward kernel per SM: 1024 threads of one vector, 512 of two; 768 of one where values are accessed
 // one by one and a row ahead takes registers.
 template <bool VEC, int LANES, int NV>
 __host__ __device__ constexpr int backward_ctas()
 {
-    const int c = VEC ? 1024 / (threads_of<LANES>() * (NV > 2 ? 4 : NV)) : (NV == 1 ? 768 : 512) / threads_of<LANES>();
+    const int c = twice<VEC, LANES, NV>() ? 512 / threads_of<LANES>()
+                : VEC ? 1024 / (threads_of<LANES>() * (NV > 2 ? 4 : NV)) : (NV == 1 ? 768 : 512) / threads_of<LANES>();
     return c < 1 ? 1 : c;
 }
 
@@ -652,6 +657,59 @@ __global__ void __launch_bounds__(threads_of<LANES>(), backward_ctas<VEC, LANES,
         statistics(row0 + stride);
         if constexpr (VEC) copies_but<R::kStages - 1>();
         else if constexpr (!kEarly) look_ahead(row0);
+        if constexpr (twice<VEC, LANES, NV>()) {
+            uint8_t* const here = mine + stage * (2 * NV * kThreads * 16);
+            const auto read = [&](int i, f2x (&h)[V / 2], f2x (&d)[V / 2]) {
+                float x[V];
+                unpack<T>(stored(here + i * (kThreads * 16)), x);
+                pairs<V>(x, h);
+                unpack<T>(stored(here + (NV + i) * (kThreads * 16)), x);
+                pairs<V>(x, d);
+#pragma unroll
+                for (int j = 0; j < V / 2; ++j) {
+                    if constexpr (!RMS) h[j] = add2(h[j], both(-mean));
+                    h[j] = mul2(h[j], both(rstd));
+                }
+            };
+            f2x s0 = 0, s1 = 0;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                if (!valid[i]) continue;
+                f2x h[V / 2], d[V / 2];
+                read(i, h, d);
+#pragma unroll
+                for (int j = 0; j < V / 2; ++j) {
+                    const f2x g = mul2(d[j], w[i].pair(j));
+                    s0 = fma2(g, h[j], s0);
+                    if constexpr (!RMS) s1 = add2(s1, g);
+                }
+            }
+            float s[kSums];
+            s[0] = sum_of(s0);
+            if constexpr (!RMS) s[1] = sum_of(s1);
+            row_sum<LANES, kSums>(s, buf, half);
+            const float c2 = s[0] * inv, c1 = RMS ? 0.0f : s[kSums - 1] * inv;
+            T* const dx = static_cast<T*>(a.y) + row * a.cols;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                if (!valid[i]) continue;
+                f2x h[V / 2], d[V / 2];
+                read(i, h, d);
+#pragma unroll
+                for (int j = 0; j < V / 2; ++j) {
+                    dw[i][j] = fma2(d[j], h[j], dw[i][j]);
+                    if constexpr (!RMS) db[i][j] = add2(db[i][j], d[j]);
+                    d[j] = mul2(d[j], w[i].pair(j));
+                    if constexpr (!RMS) d[j] = add2(d[j], both(-c1));
+                    d[j] = mul2(fma2(h[j], both(-c2), d[j]), both(rstd));
+                }
+                float x[V];
+                singles<V>(d, x);
+                if (a.y != nullptr) store<T, VEC, LANES>(dx, cols, lane, i, x);
+            }
+            stage = stage + 1 == R::kStages ? 0 : stage + 1;
+            continue;
+        }
         f2x h[NV][V / 2], g[NV][V / 2];   // the normalized values and dy w
         f2x s0 = 0, s1 = 0;
 #pragma unroll
@@ -719,7 +777,15 @@ __global__ void __launch_bounds__(threads_of<LANES>(), backward_ctas<VEC, LANES,
         float sums[NV][V];
 #pragma unroll
         for (int i = 0; i < NV; ++i) singles<V>(which ? db[i] : dw[i], sums[i]);
-        if constexpr (LANES > 32) {
+        if constexpr (LANES > 32 && VEC) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                float4* const to = reinterpret_cast<float4*>(out + which * second + column<VEC, LANES, V>(lane, i, 0));
+#pragma unroll
+                for (int k = 0; k < V / 4; ++k)
+                    if (valid[i]) to[k] = make_float4(sums[i][4 * k], sums[i][4 * k + 1], sums[i][4 * k + 2], sums[i][4 * k + 3]);
+            }
+        } else if constexpr (LANES > 32) {
 #pragma unroll
             for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -961,18 +1027,20 @@ bool vectors(const abx_norm& n, const void* second, int64_t second_stride, const
     return n.cols % v == 0 && n.x_stride % v == 0 && second_stride % v == 0 && !off(n.x, 16) && !off(second, 16) && !off(out, 16);
 }
 
-// The shape of the row kernels, by the vectors of a row: threads per row, vectors per thread.  Two vectors per thread (a
-// row of 4096 bf16 values: 256 threads) beat one (layer norm of 16384 x 4096: 49 against 63 us forward, 83 against 93
-// backward), narrow rows forward too (RMS norm of 262144 x 128: 19.8 against 21.6 us); backward these, as fast with one,
-// keep their registers.  Forward, which has no sums to hold, a bf16 row takes three or four vectors per thread where two
-// would need 512 threads (32768 x 8192: 174 against 191 us; fp32 rows are as fast with two).  Three vectors with sums spill
-// a few registers, which still beats the long kernels' second pass over x and dy (8192 x 12288 backward: 156 against 245 us;
-// 5000 x 10001: 142 against 197).
+// The shape of the row kernels, by the vectors of a row: threads per row, vectors per thread.
+//
+// Two vectors per thread (a row of 4096 bf16 values: 256 threads) beat one (layer norm of 16384 x 4096: 48 against 63 us
+// forward, 73 against 93 backward), narrow rows forward too (RMS norm of 262144 x 128: 19.8 against 21.6 us); backward these,
+// as fast with one, keep their registers.  A row of 5120 to 6144 bf16 values takes three, where two would need 512 threads
+// and one CTA per SM (RMS norm of 32768 x 5120: 154 against 191 us backward).  Of 8192 it takes four forward (32768 rows:
+// 174 against 191 us; fp32 rows are as fast with two), but not backward, where the sums leave no registers for that (343
+// against 289 us).  Longer rows take up to five vectors of 512 threads, one CTA per SM; they beat the long kernels, which
+// go through a row's memory again (5000 x 20000 bf16 values: 92 against 145 us forward, 162 against 240 backward).
 // Where values are accessed one by one, instructions count, and so do threads without a value: finer steps (8000 x 4097 in
-// bf16: 51 and 70 us against 67 and 95 with 512 threads; 100000 x 301: 39 and 58 against 44 and 57 with 64 vectors' room,
-// 54 and 81 with one vector per thread).
-// Longer rows take the long kernels.  (Sharing them among a cluster of CTAs was slower: a cluster barrier per sum and row,
-// 59 us instead of 18.5 for 515 x 20000 forward.)
+// bf16: 51 and 70 us against 67 and 95 with 512 threads; 100000 x 301: 39 and 58 against 44 and 57 with room for 64
+// vectors, 54 and 81 with one vector per thread).
+// (Sharing a long row among a cluster of CTAs was slower still: a cluster barrier per sum and row, 59 us instead of 12.6 for
+// 515 x 20000 forward.)
 template <int V, bool VEC, bool BACKWARD, typename F>
 int by_width(int64_t nvec, F&& f)
 {
@@ -995,8 +1063,15 @@ int by_width(int64_t nvec, F&& f)
             if (nvec <= 768) ABX_ROW(256, 3);
             if (nvec <= 1024) ABX_ROW(256, 4);
         }
+        if constexpr (BACKWARD) {
+            if (nvec <= 768) ABX_ROW(256, 3);
+        }
         if (nvec <= 1024) ABX_ROW(512, 2);
         if (nvec <= 1536) ABX_ROW(512, 3);
+        if constexpr (BACKWARD) {
+            if (nvec <= 2048) ABX_ROW(512, 4);
+            if (nvec <= 2560) ABX_ROW(512, 5);
+        }
     } else if constexpr (!BACKWARD) {
         if (nvec <= 48) ABX_ROW(16, 3);
         if (nvec <= 64) ABX_ROW(32, 2);
@@ -1022,6 +1097,7 @@ int by_width(int64_t nvec, F&& f)
     }
     if constexpr (!BACKWARD) {
         if (nvec <= 2048) ABX_ROW(512, 4);
+        if (nvec <= 2560) ABX_ROW(512, 5);
     }
     return f(integral_constant<int, 0>{}, integral_constant<int, 0>{});
 #undef ABX_ROW
@@ -1042,6 +1118,15 @@ int by_flags(const abx_norm& n, bool vec, F&& f)
 
 constexpr int kMaxGrid = 1 << 30;
 
+// The vectors that the backward kernel's shape goes by.  Long rows in vectors take the long kernels where they are few: a
+// CTA's sums, 8 bytes per column written and read again, are then more than what the second pass reads, 2 values per row and
+// column (300 x 12288 bf16 values 18.5 against 19.2 us, 1000 41 against 29).
+int64_t backward_vectors(const abx_norm& n, int sms, bool vec)
+{
+    const int64_t es = size_of(n.dtype), nvec = (n.cols * es + 15) / 16;
+    return vec && nvec > 1024 && n.rows * es < (int64_t)8 * sms ? INT64_MAX : nvec;
+}
+
 // Parts of the sums: a CTA of the backward kernel each, as many as are resident, or fewer when there are few
 // rows (a part is written and read again, so it should cover some).  Long rows: row runs of sums_long, so that all column
 // tiles together fill the SMs.
@@ -1049,7 +1134,7 @@ template <bool VEC>
 int backward_parts(const abx_norm& n, int sms)
 {
     const int64_t v = 16 / size_of(n.dtype), nvec = (n.cols + v - 1) / v;
-    return by_width<8, VEC, true>(nvec, [&](auto lanes, auto nv) {
+    return by_width<8, VEC, true>(backward_vectors(n, sms, VEC), [&](auto lanes, auto nv) {
         constexpr int L = decltype(lanes)::value, NV = decltype(nv)::value;
         if constexpr (L == 0) {
             const int64_t tiles = (nvec + 31) / 32, want = (8 * sms + tiles - 1) / tiles, most = (n.rows + 31) / 32;
@@ -1162,7 +1247,7 @@ ABX_API int abx_norm_backward(void* stream, const abx_norm* norm, const void* dy
         using W = decltype(weight);
         constexpr bool kRms = decltype(rms)::value, kVec = decltype(vec)::value;
         const int64_t nvec = (n.cols + Vec<T>::V - 1) / Vec<T>::V;
-        return by_width<Vec<T>::V, kVec, true>(nvec, [&](auto lanes, auto nv) {
+        return by_width<Vec<T>::V, kVec, true>(backward_vectors(n, sms, kVec), [&](auto lanes, auto nv) {
             constexpr int L = decltype(lanes)::value, NV = decltype(nv)::value;
             if constexpr (L == 0) {
                 if (dx && n.rows > 0) {
