@@ -857,14 +857,21 @@ int check(const abx_graph_tensor& t, const abx_graph_step& h)
     return ABX_OK;
 }
 
-int resident_ctas(const void* kernel, int* out)
+// CTAs of a kernel that are resident on the current device, asked for once per device.
+template <auto KERNEL>
+int resident_ctas(int* out)
 {
+    constexpr int kDevices = 64;
+    static std::atomic<int> known[kDevices];
     int dev = 0, sms = 0, per = 0;
     cudaError_t e = cudaGetDevice(&dev);
+    const bool keep = e == cudaSuccess && dev < kDevices;
+    if (keep && (*out = known[dev].load(std::memory_order_relaxed)) > 0) return ABX_OK;
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, kThreads, 0);
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, (const void*)KERNEL, kThreads, 0);
     if (e != cudaSuccess) return abx::set_error("launch geometry", e);
     *out = sms * (per > 0 ? per : 1);
+    if (keep) known[dev].store(*out, std::memory_order_relaxed);
     return ABX_OK;
 }
 
@@ -872,7 +879,7 @@ template <bool I8, bool SR, typename W, int N>
 int launch_step(const Args<N>& a, int32_t max_ctas, cudaStream_t st)
 {
     int grid = 0;
-    if (int rc = resident_ctas((const void*)step_kernel<I8, SR, W, N>, &grid)) return rc;
+    if (int rc = resident_ctas<step_kernel<I8, SR, W, N>>(&grid)) return rc;
     if (grid > a.tiles) grid = a.tiles;
     if (max_ctas > 0 && grid > max_ctas) grid = max_ctas;
     step_kernel<I8, SR, W, N><<<grid, kThreads, 0, st>>>(a);
@@ -931,7 +938,7 @@ int i8_run(void* stream, void* codes, float* scales, float* values, int64_t n, i
     if (n == 0) return ABX_OK;
     const I8Args a{codes, scales, values, n, (n + kBlock - 1) / kBlock, -0.0f};
     int grid = 0;
-    if (int rc = resident_ctas(role ? (const void*)KV : (const void*)KM, &grid)) return rc;
+    if (int rc = role ? resident_ctas<KV>(&grid) : resident_ctas<KM>(&grid)) return rc;
     const int64_t need = (a.blocks + kWarps * at_once - 1) / (kWarps * at_once);
     if (need < grid) grid = (int)need;
     if (role) KV<<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
