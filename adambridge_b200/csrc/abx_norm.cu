@@ -464,8 +464,9 @@ __global__ void __launch_bounds__(threads_of<LANES>()) forward_kernel(const __gr
     }
 }
 
-// Rows longer than a CTA's registers (more than 2560 vectors): three passes over the row, which is kept in shared memory where it fits and rows
-// allow vector access (each thread copies and reads its own vectors), and read again from the caches where not.
+// Rows longer than a CTA's registers (and backward, long rows that are few): three passes over the row, which is kept in
+// shared memory where it fits and rows allow vector access (each thread copies and reads its own vectors), and read again
+// from the caches where not.
 constexpr int kLong = 512;
 
 // A thread's vector i of the row, of `count` rows of one image each (x, or x and dy).

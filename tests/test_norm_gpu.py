@@ -101,6 +101,15 @@ def test_every_row_shape(cols, dtype, rms):
         check(x, w, None if rms else b, 1e-5, rms, dy)
 
 
+@pytest.mark.parametrize("cols", [2056, 4104, 5120, 6144, 6152, 9001, 10240, 10248, 12296, 15001, 16392, 20480, 20488])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_many_long_rows(cols, dtype):
+    """Enough long rows that each CTA takes several and keeps their sums, which the shapes for long rows need."""
+    x, w, b, dy = data(700, cols, dtype, cols)
+    check(x, w, b, 1e-5, False, dy)
+    check(x.detach(), w.detach(), None, 1e-5, True, dy, (cols % 16 == 0, True, False))
+
+
 @pytest.mark.parametrize("xt, wt", [(torch.bfloat16, torch.float32), (torch.float32, torch.bfloat16)])
 @pytest.mark.parametrize("cols", [64, 129, 4096, 4100, 20000])
 def test_mixed_types(xt, wt, cols):
