@@ -61,7 +61,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         return LIB
     LIBDIR.mkdir(exist_ok=True)
     tmp = LIBDIR / f".libabx.{os.getpid()}.so"
-    cmd = [nvcc(), *ARCH, *FLAGS, *(["-Xptxas", "-v"] if verbose else []), "-I", str(INCLUDE),
+    cmd = [nvcc(), *ARCH, *FLAGS, "--threads", "0", *(["-Xptxas", "-v"] if verbose else []), "-I", str(INCLUDE),
            *map(str, SOURCES), "-o", str(tmp)]
     if verbose:
         print(" ".join(cmd), file=sys.stderr)
