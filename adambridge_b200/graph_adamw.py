@@ -148,6 +148,22 @@ class StateArena:
             return {"precision": "int8", "role": role, "block": BLOCK, "q": codes, "scale": scale}
         return {"precision": "fp32", "data": self._ops.i8_decode(codes, scale, n, role == "v")}
 
+    def reset_master(self, i: int) -> None:
+        """Parameter ``i``'s master from its weight as it is now."""
+        if self.master_offsets[i] is not None:
+            self.master_of(i).copy_(self.params[i].detach().reshape(-1))
+
+    def reset(self, i: int) -> None:
+        """Parameter ``i``'s state as a new optimizer has it, in place."""
+        at, end = self.offsets[i], self.offsets[i] + _padded(self.numels[i])
+        self.m[at:end].zero_()
+        self.v[at:end].zero_()
+        if self.m_scale is not None:
+            self.m_scale[at // BLOCK:end // BLOCK].zero_()
+            self.v_scale[at // BLOCK:end // BLOCK].zero_()
+        self.steps[i] = 0
+        self.reset_master(i)
+
     def load_moment(self, i: int, role: str, saved: "dict | StateBuffer") -> None:
         """Write a checked checkpoint moment: int8 planes as they are, other formats by their values."""
         plane, scales = self._plane(role)
@@ -379,7 +395,10 @@ class GraphAdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def load_state_dict(self, state_dict: dict[str, Any]) -> None:
         """Load a GraphAdamW, AdamBridge or ``torch.optim.AdamW`` checkpoint.  Everything is checked before anything
-        changes; moments in another format are re-encoded on the GPU (to the nearest codes)."""
+        changes; moments in another format are re-encoded on the GPU (to the nearest codes).
+
+        The checkpoint replaces the whole state, in the same buffers: a parameter that it does not list starts over, and
+        an fp32 master that it does not hold is taken from the bf16 weight, so load the model's weights first."""
         where = [(arena, i) for arena in self.prepare().arenas for i in range(len(arena.params))]
         parsed = {}
         for key, entry in state_dict["state"].items():
@@ -413,10 +432,15 @@ class GraphAdamW(torch.optim.Optimizer):
         for group, lr in zip(self.param_groups, rates):
             if isinstance(lr, torch.Tensor):   # a captured step reads this tensor
                 group["lr"] = lr.copy_(torch.as_tensor(group["lr"]).reshape(lr.shape))
-        for index, (step, master, found) in parsed.items():
-            arena, i = where[index]
+        for index, (arena, i) in enumerate(where):
+            if index not in parsed:
+                arena.reset(i)
+                continue
+            step, master, found = parsed[index]
             arena.steps[i] = step
             if master is not None:
                 arena.master_of(i).copy_(master.to_device(arena.device).to_fp32())
+            else:
+                arena.reset_master(i)
             for role, saved in found:
                 arena.load_moment(i, role, saved)

@@ -548,6 +548,64 @@ def test_bad_checkpoints_change_nothing(change, message):
     assert all(torch.equal(a, b) for a, b in zip(before, snapshot(params, opt)))
 
 
+@pytest.mark.parametrize("precision", ["fp32", "int8"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_checkpoint_replaces_the_whole_state(precision, dtype):
+    """Saved before the first step and loaded after some: what a new optimizer on the same weights has, in the same
+    buffers, which captured graphs address."""
+    params, opt = make([5000, 300, 7], dtype, 3, precision=precision)
+    weights = [p.detach().clone() for p in params]
+    saved = torch.load(_saved(opt), weights_only=True)
+    for _ in range(3):
+        opt.step()
+    buffers = lambda: [t.data_ptr() for t in (opt.arenas[0].m, opt.arenas[0].v, opt.arenas[0].steps)]   # noqa: E731
+    where = buffers()
+    for p, w in zip(params, weights):
+        p.data.copy_(w)
+    opt.load_state_dict(saved)
+    fresh, new = make([5000, 300, 7], dtype, 3, precision=precision)
+    new.prepare()
+    assert all(torch.equal(a, b) for a, b in zip(snapshot(params, opt), snapshot(fresh, new)))
+    assert buffers() == where
+    for o in (opt, new):
+        o.step()
+    assert all(torch.equal(a, b) for a, b in zip(snapshot(params, opt), snapshot(fresh, new)))
+
+
+@pytest.mark.parametrize("precision", ["fp32", "int8"])
+def test_a_parameter_that_a_checkpoint_lacks_starts_over(precision):
+    params, opt = make([5000, 300, 7], torch.bfloat16, 3, precision=precision)
+    lacking, partial = make([5000, 300, 7], torch.bfloat16, 3, precision=precision)
+    lacking[1].grad = None
+    for _ in range(2):
+        opt.step()
+        partial.step()
+    assert sorted(partial.state_dict()["state"]) == [0, 2]
+    for p, w in zip(params, lacking):
+        p.data.copy_(w)
+    opt.load_state_dict(torch.load(_saved(partial), weights_only=True))
+    assert all(torch.equal(a, b) for a, b in zip(snapshot(params, opt), snapshot(lacking, partial)))
+
+
+def test_masters_follow_the_weights_where_a_checkpoint_has_none():
+    """A torch.optim.AdamW checkpoint with the bf16 weights saved beside it, loaded after the state was made from others."""
+    source, _ = make([5000, 300], torch.bfloat16, 4)
+    ref = torch.optim.AdamW(source, lr=1e-3)
+    ref.step()
+    params, opt = make([5000, 300], torch.bfloat16, 3, precision="fp32")
+    opt.step()
+    for p, s in zip(params, source):
+        p.data.copy_(s)
+    opt.load_state_dict(ref.state_dict())
+    for i, s in enumerate(source):
+        assert torch.equal(opt.arenas[0].master_of(i), s.detach().float())
+    assert opt.arenas[0].steps.tolist() == [1, 1]
+    for group in opt.param_groups:
+        group.update(lr=0.0)
+    opt.step()
+    assert all(torch.equal(p, s) for p, s in zip(params, source))
+
+
 # --------------------------------------------------------------------------- refusals
 
 def test_refusals():
