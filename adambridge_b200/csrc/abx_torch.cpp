@@ -187,7 +187,7 @@ Tensor norm(const Tensor& x, const std::optional<Tensor>& weight, const std::opt
 // The kernel descriptions of one arena's parameters that have a gradient, with the tensors they point at.
 struct Described {
     std::vector<abx_graph_tensor> tensors;
-    std::vector<Tensor> keep;
+    std::vector<Tensor> params, keep;
     c10::Device device{c10::kCUDA, 0};
 };
 
@@ -200,6 +200,7 @@ std::unique_ptr<Described> describe_step(const std::vector<Tensor>& params, cons
     auto d = std::make_unique<Described>();
     d->device = c10::Device(c10::kCUDA, (c10::DeviceIndex)device);
     d->tensors.reserve(params.size());
+    d->params.reserve(params.size());
     d->keep.reserve(params.size());
     const auto* row = reinterpret_cast<const abx_graph_tensor*>(rows.const_data_ptr());
     for (size_t i = 0; i < params.size(); ++i, ++row) {
@@ -224,6 +225,7 @@ std::unique_ptr<Described> describe_step(const std::vector<Tensor>& params, cons
         t.w = p.data_ptr();
         t.g = g.const_data_ptr();
         d->tensors.push_back(t);
+        d->params.push_back(p);
         d->keep.push_back(std::move(g));
     }
     return d;
@@ -239,6 +241,9 @@ void launch_step(const Described& d, uintptr_t shared, const Tensor& ticket, int
     succeeded(abx_graph_adamw(stream_of(ticket), d.tensors.data(), (int32_t)d.tensors.size(),
                               reinterpret_cast<const abx_graph_step*>(shared), reinterpret_cast<uint32_t*>(ticket.data_ptr()),
                               (int32_t)max_ctas), "abx_graph_adamw");
+    // as an operation in place says to autograd: a graph that saved a weight may no longer run backward
+    for (const Tensor& p : d.params)
+        if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
 }
 
 // ---- 8-bit moments -----------------------------------------------------------------------------------

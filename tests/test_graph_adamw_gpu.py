@@ -455,6 +455,21 @@ def test_agrees_with_adambridge(dtype):
         assert float((a - b.view(-1)).abs().max()) <= 5 * E * (3 * 0.1 + 16 * 1e-2)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_step_between_forward_and_backward_is_noticed(dtype):
+    """As torch's optimizers: the backward pass of a graph that saved a weight fails once a step has changed it."""
+    params, opt = make([64, 300, 64], dtype, 1)
+    params[1].grad = None
+    before = [p._version for p in params]
+    x = torch.randn(5, 64, device="cuda", dtype=dtype, requires_grad=True)
+    kept, other = ab.rms_norm(x, params[0]), ab.rms_norm(x, params[2].detach().clone())
+    opt.step()
+    assert [p._version > b for p, b in zip(params, before)] == [True, False, True]
+    other.sum().backward()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        kept.sum().backward()
+
+
 # --------------------------------------------------------------------------- checkpoints
 
 @pytest.mark.parametrize("precision", ["fp32", "int8"])
