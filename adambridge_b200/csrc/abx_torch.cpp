@@ -7,11 +7,13 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <ATen/ATen.h>
 #include <ATen/TensorUtils.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAStream.h>
 
 #include <memory>
@@ -115,6 +117,12 @@ std::tuple<Tensor, Tensor, Tensor> forward_norm(const Tensor& x, const std::opti
     return {y, rows.t, stats};
 }
 
+// Level 0 is torch's only one.
+void check_tangent(const Tensor& t)
+{
+    TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), "layer_norm and rms_norm have no forward-mode derivatives");
+}
+
 class Norm : public torch::autograd::Function<Norm> {
 public:
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& weight,
@@ -133,6 +141,7 @@ public:
         const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &stats = saved[3], &dy = grads[0];
         variable_list out(5);
         if (!dy.defined()) return out;
+        check_tangent(dy);
         // edges are counted over the tensors that were given
         const bool want_x = ctx->needs_input_grad(0);
         const bool want_w = weight.defined() && ctx->needs_input_grad(1);
@@ -174,9 +183,24 @@ public:
     }
 };
 
+// What follows a program through torch's dispatcher does not see a norm: it would take the result for one that nothing
+// computes, or for one that does not depend on x.
+void check_seen(const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias)
+{
+    using Mode = c10::impl::TorchDispatchModeKey;
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing()
+                                    && !c10::impl::TorchDispatchModeTLS::get_mode(Mode::PROXY)
+                                    && !c10::impl::TorchDispatchModeTLS::get_mode(Mode::FAKE),
+                                "layer_norm and rms_norm are not operators of torch's dispatcher: a trace does not see them");
+    check_tangent(x);
+    if (weight) check_tangent(*weight);
+    if (bias) check_tangent(*bias);
+}
+
 Tensor norm(const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, double eps, bool rms)
 {
     check_norm(x, weight, bias, eps);
+    check_seen(x, weight, bias);
     if (at::GradMode::is_enabled() && (x.requires_grad() || (weight && weight->requires_grad()) || (bias && bias->requires_grad())))
         return Norm::apply(x, weight, bias, eps, rms);
     return std::get<0>(forward_norm(x, weight, bias, eps, rms, false));

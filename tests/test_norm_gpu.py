@@ -323,6 +323,44 @@ def test_refusals():
         g.sum().backward()
 
 
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(which, grad):
+    """A tangent that went nowhere would read as a derivative of 0."""
+    import torch.autograd.forward_ad as forward_ad
+    args = [t.detach() for t in data(4, 64, torch.float32)[:3]]
+    args[0].requires_grad_(grad)
+    with forward_ad.dual_level():
+        args[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            ab.layer_norm(*args)
+        if which < 2:
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                ab.rms_norm(*args[:2])
+    x, w, _, dy = data(4, 64, torch.float32)
+    y = ab.rms_norm(x.requires_grad_(True), w)
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        torch.autograd.grad(y, x, forward_ad.make_dual(dy, torch.ones_like(dy)))
+
+
+def test_traces_and_transforms_are_refused():
+    """They would record a result that nothing computes, or cannot reach the values."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, w, b, _ = data(4, 64, torch.float32)
+    for fn in (lambda t: ab.layer_norm(t, w, b), lambda t: ab.rms_norm(t, w)):
+        with pytest.raises(Exception, match="trace does not see"):
+            torch.jit.trace(fn, (x,))
+        with pytest.raises(NotImplementedError, match="trace does not see"):
+            make_fx(fn)(x)
+        with pytest.raises(NotImplementedError, match="trace does not see"), FakeTensorMode(allow_non_fake_inputs=True) as mode:
+            fn(mode.from_tensor(x))
+        for transformed in (torch.func.vmap(fn), torch.func.grad(lambda t: fn(t).sum()),
+                            lambda t: torch.func.jvp(fn, (t,), (torch.ones_like(t),))):
+            with pytest.raises(RuntimeError):
+                transformed(x)
+
+
 # --------------------------------------------------------------------------- a training step of these operators
 
 class Net(torch.nn.Module):
