@@ -230,7 +230,8 @@ class GraphAdamW(torch.optim.Optimizer):
         self.precision, self.stochastic, self.seed, self.max_ctas = precision, stochastic_rounding, seed, max_ctas
         self.arenas: list[StateArena] = []       # one per parameter group, once prepared
         self._native = native.load()
-        self._clip: tuple[torch.Tensor, torch.Tensor, bool] | None = None   # coefficient, norm, captured
+        # coefficient, norm, captured, the stream that they were made on
+        self._clip: tuple[torch.Tensor, torch.Tensor, bool, torch.cuda.Stream] | None = None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
     def add_param_group(self, param_group: dict[str, Any]) -> None:
@@ -302,6 +303,11 @@ class GraphAdamW(torch.optim.Optimizer):
                 for arena, group in zip(self.arenas, self.param_groups)]
         for arena, described, shared in work:
             arena.launch(described, shared, self.max_ctas)
+        if clip is not None:
+            made, now = clip[3], torch.cuda.current_stream(clip[3].device)
+            if now != made:   # the memory stays until this stream has read it
+                for t in clip[:2]:
+                    t.record_stream(now)
         return loss
 
     def _shared(self, arena: StateArena, group: dict[str, Any], coef, found_inf, norm) -> native.GraphStep:
@@ -351,7 +357,7 @@ class GraphAdamW(torch.optim.Optimizer):
             norms = [clip_coefficient(part, max_norm, kernels=self._native)[2] for part in parts]
             total = torch.linalg.vector_norm(torch.cat(norms))
             coef = torch.clamp(max_norm / (total + 1e-6), max=1.0).reshape(1)
-        self._clip = (coef, total.float().reshape(1), _capturing())
+        self._clip = (coef, total.float().reshape(1), _capturing(), torch.cuda.current_stream(grads[0].device))
         return total
 
     # ------------------------------------------------------------------ inspection

@@ -470,6 +470,32 @@ def test_a_step_between_forward_and_backward_is_noticed(dtype):
         kept.sum().backward()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_clip_on_one_stream_and_its_step_on_another(dtype):
+    """The coefficient stays until the step has read it, although the clip's stream goes on and takes free memory."""
+    def build():
+        params, opt = make([300, 5000], dtype, 6, precision="fp32")
+        return params, opt.prepare()
+
+    params, opt = build()
+    want, plain = build()
+    plain.clip_grad_norm_(1e-3)
+    plain.step()
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(one):
+        opt.clip_grad_norm_(1e-3)
+    two.wait_stream(one)
+    with torch.cuda.stream(two):
+        torch.cuda._sleep(50_000_000)        # some 30 ms
+        opt.step()
+    with torch.cuda.stream(one):
+        taken = [torch.full((k,), 1e6, device="cuda") for k in (1, 2, 4) for _ in range(32)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(snapshot(params, opt), snapshot(want, plain)))
+    del taken
+
+
 # --------------------------------------------------------------------------- checkpoints
 
 @pytest.mark.parametrize("precision", ["fp32", "int8"])
