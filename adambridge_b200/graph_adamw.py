@@ -342,6 +342,7 @@ class GraphAdamW(torch.optim.Optimizer):
         step is skipped on the device if it is not finite."""
         if float(norm_type) != 2.0:
             raise ValueError("GraphAdamW.clip_grad_norm_ computes the L2 norm (norm_type=2) only")
+        self._clip = None
         grads = [p.grad for group in self.param_groups for p in group["params"] if p.grad is not None]
         if not grads:
             return torch.tensor(0.0)

@@ -496,6 +496,20 @@ def test_a_clip_on_one_stream_and_its_step_on_another(dtype):
     del taken
 
 
+def test_a_clip_without_gradients_takes_the_last_one_back():
+    params, opt = make([300], torch.float32, 6, precision="fp32")
+    other, plain = make([300], torch.float32, 6, precision="fp32")
+    opt.clip_grad_norm_(1e-3)
+    grads = [p.grad for p in params]
+    opt.zero_grad(set_to_none=True)
+    assert float(opt.clip_grad_norm_(1e-3)) == 0.0
+    for p, g in zip(params, grads):
+        p.grad = g
+    opt.step()
+    plain.step()
+    assert all(torch.equal(a, b) for a, b in zip(params, other))
+
+
 # --------------------------------------------------------------------------- checkpoints
 
 @pytest.mark.parametrize("precision", ["fp32", "int8"])
