@@ -47,8 +47,9 @@ struct Rows {
     int64_t stride;    // elements between rows
 };
 
-Rows rows_of(const Tensor& t)
+Rows rows_of(const Tensor& given)
 {
+    const Tensor t = given.resolve_neg();   // memory of a lazily negated view holds the other sign
     const int64_t cols = t.size(-1);
     if (!t.is_contiguous()) {
         const int64_t count = t.numel() / cols;
@@ -96,7 +97,8 @@ abx_norm describe(const Rows& x, const Tensor& weight, const Tensor& bias, doubl
     return n;
 }
 
-Tensor contiguous(const std::optional<Tensor>& t) { return t ? t->contiguous() : Tensor(); }
+Tensor contiguous(const Tensor& t) { return t.defined() ? t.resolve_neg().contiguous() : t; }
+Tensor contiguous(const std::optional<Tensor>& t) { return contiguous(t.value_or(Tensor())); }
 
 // y, x as the kernels read it, and where `keep`, the rows' statistics: rstd, then the mean (not for RMS norm)
 std::tuple<Tensor, Tensor, Tensor> forward_norm(const Tensor& x, const std::optional<Tensor>& weight,
@@ -152,7 +154,7 @@ public:
             const c10::DeviceGuard guard(x.device());
             const bool rms = ctx->saved_data["rms"].toBool();
             const Rows rows = rows_of(x), given = rows_of(dy);
-            const Tensor w = weight.defined() ? weight.contiguous() : weight, b = bias.defined() ? bias.contiguous() : bias;
+            const Tensor w = contiguous(weight), b = contiguous(bias);
             const abx_norm n = describe(rows, w, b, ctx->saved_data["eps"].toDouble(), rms);
             if (want_x) out[0] = at::empty(x.sizes(), x.options());
             if (want_w) out[1] = at::empty(weight.sizes(), weight.options());
@@ -235,15 +237,15 @@ std::unique_ptr<Described> describe_step(const std::vector<Tensor>& params, cons
                         && p.device() == d->device,
                     "a parameter changed after its state was made (", row->n, " values of dtype code ", row->dtype, " on ",
                     d->device, ", now ", p.numel(), " x ", p.scalar_type(), " on ", p.device(), ")");
-        TORCH_CHECK_VALUE(p.is_contiguous(), "non-contiguous parameters are not supported");
+        TORCH_CHECK_VALUE(p.is_contiguous() && !p.is_neg(), "non-contiguous parameters are not supported, nor negated views");
         TORCH_CHECK(!g.is_sparse() && g.layout() == at::kStrided, "GraphAdamW does not support sparse gradients");
         TORCH_CHECK_TYPE(g.scalar_type() == p.scalar_type(), "the gradient of a ", p.scalar_type(), " parameter must be ",
                          p.scalar_type(), ", got ", g.scalar_type());
         TORCH_CHECK_VALUE(g.numel() == row->n && g.device() == d->device, "a gradient has ", g.numel(), " elements on ",
                           g.device(), ", its parameter ", row->n, " on ", d->device);
-        if (!g.is_contiguous()) {
+        if (!g.is_contiguous() || g.is_neg()) {
             const c10::DeviceGuard guard(d->device);
-            g = g.contiguous();
+            g = g.resolve_neg().contiguous();
         }
         abx_graph_tensor t = *row;
         t.w = p.data_ptr();

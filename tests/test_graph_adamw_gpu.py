@@ -215,6 +215,18 @@ def test_unaligned_strided_and_neighbours(precision, dtype):
     assert torch.equal(one.arenas[0].exp_avg(), two.arenas[0].exp_avg())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_negated_gradients(dtype):
+    """A gradient that is a lazily negated view, as the imaginary part of a conjugate is."""
+    (params, opt), (other, plain) = (make([300, 5000], dtype, 3, precision="fp32") for _ in range(2))
+    for p, o in zip(params, other):
+        p.grad = torch._neg_view(p.grad.clone())
+        o.grad.neg_()
+    opt.step()
+    plain.step()
+    assert all(torch.equal(a, b) for a, b in zip(params, other))
+
+
 def test_missing_gradients_and_mixed_types():
     bf, _ = make([300, 40, 513], torch.bfloat16, 1)
     fp, _ = make([77, 1000], torch.float32, 2)

@@ -161,6 +161,23 @@ def test_strides(cols, dtype):
     assert torch.equal(wide, keep)
 
 
+@pytest.mark.parametrize("which", ["x", "w", "b", "dy"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_negated_views(which, dtype):
+    """Lazily negated tensors, as the imaginary part of a conjugate is, give what negated copies give."""
+    given = dict(zip("x w b dy".split(), data(50, 72, dtype, 4)))
+    lazy = dict(given, **{which: torch._neg_view(given[which])})
+    given[which] = -given[which]
+    results = []
+    for t in (given, lazy):
+        leaves = [t[k].requires_grad_(True) for k in ("x", "w", "b")]
+        y = ab.layer_norm(*leaves)
+        results.append([y, *torch.autograd.grad(y, leaves, t["dy"])])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    z = torch.randn(300, 1, dtype=torch.complex64, device="cuda").conj().imag
+    assert z.is_neg() and torch.equal(ab.rms_norm(z), ab.rms_norm(z.clone()))
+
+
 @pytest.mark.parametrize("cols", [1, 3, 9, 33, 61, 121, 129, 250, 505, 1001, 2050, 4097, 5121, 8185, 9001, 17001, 20003])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_rows_between_other_data(dtype, cols):
