@@ -83,7 +83,8 @@ struct Args {
     uint32_t seed;
     float b1, omb1, b2, omb2, eps;
     float minus_zero;
-    uint32_t zero_is_plain;   // eps is in [2^-60, 2^60]: v = 0 needs no IEEE division
+    uint32_t plain_low, plain_high;   // v's bits for which the fast root and quotient are the IEEE ones (v in [low, high))
+    uint32_t zero_is_plain;   // so they are for v = 0
     Item t[N];
 };
 
@@ -255,9 +256,11 @@ __device__ __forceinline__ f2x first_of(f2x x, int n)
 // Root and quotient by Newton's iteration from the hardware's approximations, with Markstein's last step: the exact
 // remainder by FMA, times the reciprocal, added to the approximation, rounds correctly (P. Markstein, IBM J. Res.
 // Dev. 34(1), 1990).  In pairs that is a third of the instructions of the scalar IEEE operations, which otherwise
-// take a quarter of the kernel.  The root equals __fsqrt_rn for every float of [2^-100, 2^120) and for 0; the
-// quotient equalled __fdiv_rn for 7.7e10 random operands, |x| above 2^-100 and the divisor in [2^-60, 2^90].
-// Outside (see `plain` in step_kernel) the IEEE operations are used.
+// take a quarter of the kernel.  The remainder has to be exact, a multiple of 2^-149, and the quotient a normal number:
+// `update` uses them for a second moment that is 0 or in [2^-100, 2^48 (1 - b2)), a first one that is 0 or at least 2^-100
+// and a divisor of [2^-60, 2^25], and the IEEE operations for a lane's eight values where one is outside.  (A first moment of 2^64 or
+// more, which no step leaves beside such a second one, has no test of its own.)  The tests compare every float as a root's
+// operand, and quotients of moments from 2^-149 on, with results in 64 bits.
 __device__ __forceinline__ f2x sqrt2(f2x x)
 {
     float a, b, ya, yb;
@@ -471,7 +474,7 @@ struct Lane {
 struct Constants {
     float scale, b1, omb1, b2, omb2, eps;
     f2x minus_zero;
-    uint32_t zero_is_plain;
+    uint32_t plain_low, plain_high, zero_is_plain;
 };
 
 // Eight values of a lane as they are stored.
@@ -500,6 +503,15 @@ __device__ __forceinline__ void load(Loaded<I8, W>& x, const Lane<I8, W>& t, int
     }
 }
 
+__device__ __forceinline__ float least_abs(float a, float b, float c)
+{
+    float d;
+    asm("min.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+constexpr float kLeastPlain = 0x1p-100f;   // of a first moment that is not 0, and of a second one
+
 // One block of 256 values, 8 per lane.
 template <bool I8, bool SR, bool FULL, typename W>
 __device__ __forceinline__ void update(const Loaded<I8, W>& in, const Lane<I8, W>& t, const Constants& k, const StepCoef& c,
@@ -519,6 +531,7 @@ __device__ __forceinline__ void update(const Loaded<I8, W>& in, const Lane<I8, W
         pairs(in.v, v);
     }
     uint32_t low = 0xffffffffU, high = 0;   // the extremes of v's bits
+    float least = 1.0f;                     // ... and of |m|
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const f2x gj = mul2(g[j], both(k.scale));
@@ -528,18 +541,23 @@ __device__ __forceinline__ void update(const Loaded<I8, W>& in, const Lane<I8, W
         up2(v[j], v0, v1);
         low = __vimin3_u32(low, f2u(v0), f2u(v1));
         high = __vimax3_u32(high, f2u(v0), f2u(v1));
+        float m0, m1;
+        up2(m[j], m0, m1);
+        least = least_abs(least, m0, m1);
         root[j] = sqrt2(v[j]);
         q[j] = quotient2(m[j], add2(term2(root[j], both(c.inv_sqrt_bc2), nz), both(k.eps)));
     }
     uint32_t zeros[2] = {0, 0};   // a 1 in the byte of each v that is 0
-    if (__builtin_expect(low < 0x0e000000U || high >= 0x7b800000U, 0)) {   // under 2^-99 or not under 2^120
-        bool ieee = !k.zero_is_plain || high >= 0x7b800000U;
+    if (__builtin_expect(low < k.plain_low || high >= k.plain_high || least < kLeastPlain, 0)) {
+        bool ieee = !k.zero_is_plain || high >= k.plain_high;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            float v0, v1;
+            float v0, v1, m0, m1;
             up2(v[j], v0, v1);
+            up2(m[j], m0, m1);
             zeros[j >> 1] |= ((f2u(v0) == 0 ? 1U : 0U) | (f2u(v1) == 0 ? 0x100U : 0U)) << (16 * (j & 1));
-            ieee |= (f2u(v0) != 0 && f2u(v0) < 0x0e000000U) || (f2u(v1) != 0 && f2u(v1) < 0x0e000000U);
+            ieee |= (f2u(v0) != 0 && f2u(v0) < k.plain_low) || (f2u(v1) != 0 && f2u(v1) < k.plain_low)
+                    || (m0 != 0.0f && fabsf(m0) < kLeastPlain) || (m1 != 0.0f && fabsf(m1) < kLeastPlain);
         }
         if (ieee) {
 #pragma unroll
@@ -694,7 +712,8 @@ __global__ void __launch_bounds__(kThreads, kStepCtas<I8>) step_kernel(const __g
     // skip is a flag as loss scalers write it; a norm that is not finite says the same of the gradients
     if (a.skip != nullptr && !(*a.skip == 0.0f)) return;
     if (a.norm != nullptr && !(fabsf(*a.norm) <= 3.402823466e38f)) return;
-    const Constants constants{a.g_scale != nullptr ? *a.g_scale : 1.0f, a.b1, a.omb1, a.b2, a.omb2, a.eps, both(a.minus_zero), a.zero_is_plain};
+    const Constants constants{a.g_scale != nullptr ? *a.g_scale : 1.0f, a.b1, a.omb1, a.b2, a.omb2, a.eps, both(a.minus_zero),
+                              a.plain_low, a.plain_high, a.zero_is_plain};
     const uint32_t mine = threadIdx.x / 32 * kBlock;   // the warp's block in a tile
     uint8_t* const slots = ring + threadIdx.x / 32 * (R::kStages * R::kBytes);
     const int64_t apart = (int64_t)gridDim.x * kTile;
@@ -903,7 +922,12 @@ int run_batch(const abx_graph_tensor* t, const int32_t* order, int32_t count, co
     a.b2 = (float)h.beta2; a.omb2 = (float)(1.0 - h.beta2);
     a.eps = (float)h.eps;
     a.minus_zero = -0.0f;
-    a.zero_is_plain = a.eps >= 0x1p-60f && a.eps <= 0x1p60f;
+    // The divisor is sqrt(v) c + eps, c at most 1 / sqrt(1 - b2): below 2^24 + 2^24 where v is below 2^48 (1 - b2).
+    const float high = (float)((1.0 - h.beta2) * 0x1p48), low = kLeastPlain;
+    std::memcpy(&a.plain_low, &low, 4);
+    std::memcpy(&a.plain_high, &high, 4);
+    if (a.eps > 0x1p24f) a.plain_high = 0;
+    a.zero_is_plain = a.eps >= 0x1p-60f;
     int64_t next = 0;
     for (int32_t j = 0; j < count; ++j) {
         const abx_graph_tensor& s = t[order[j]];

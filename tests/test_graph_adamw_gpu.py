@@ -144,6 +144,71 @@ def test_against_64_bits(dtype, precision, stochastic, spread):
         assert bool(((gv.double().sqrt() - v1.sqrt()).abs() <= off_r + 2 * E * v1.sqrt()).all())
 
 
+def plain_step(m, v, eps):
+    """One fp32 step with zero gradients from the moments m, v.  Decays of 1/2 halve them, after 200 steps the bias
+    corrections are 1, and the learning rate is 1: a weight of 0 becomes -(m' / (sqrt(v') + eps)).  Returns that and what
+    64 bits say, rounded once at each operation (a root or quotient of two floats in 53 bits rounds to the right one)."""
+    p = torch.nn.Parameter(torch.zeros_like(m))
+    p.grad = torch.zeros_like(m)
+    opt = ab.GraphAdamW([p], lr=1.0, betas=(0.5, 0.5), eps=eps, weight_decay=0.0, precision="fp32").prepare()
+    a, n = opt.arenas[0], m.numel()
+    a.m[:n].copy_(m)
+    a.v[:n].copy_(v)
+    a.steps.fill_(200)
+    opt.step()
+    m, v = a.m[:n], a.v[:n]
+    d = v.double().sqrt().float() + torch.tensor(eps, dtype=torch.float32, device="cuda")
+    return p.detach(), -(m.double() / d.double()).float()
+
+
+def test_roots_of_every_second_moment():
+    """Every float of [2^-104, 2^50), which is what the fast root takes and some of what it does not on either side."""
+    start, stop, at_once = 23 << 23, 177 << 23, 1 << 26
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    for at in range(start, stop, at_once):
+        bits = torch.arange(at, min(at + at_once, stop), dtype=torch.int32, device="cuda")
+        v = bits.view(torch.float32) * 2
+        got, want = plain_step(torch.empty_like(v).uniform_(0.5, 2.0, generator=gen), v, 0.0)
+        assert torch.equal(got, want), at
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 1e-8, 1.0, 2.0 ** 24, 2.0 ** 40, 2.0 ** 100])
+@pytest.mark.parametrize("low, high", [(-149, -100), (-149, 60), (-101, 0)])
+def test_quotients_of_first_moments_of_any_size(low, high, eps):
+    """First moments that decayed to 2^-149 beside second moments of any size, zeros among both: the quotient is the IEEE
+    one, also where it or the remainder that corrects it leaves the range of normal numbers."""
+    n = (1 << 22) + 1000
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    def spread(a, b):
+        e = torch.empty(n, device="cuda", dtype=torch.float64).uniform_(a, b, generator=gen)
+        return torch.exp2(e).float()
+    m, v = spread(low, high), spread(-140, 120)
+    m *= torch.where(torch.rand(n, device="cuda", generator=gen) < 0.5, -1.0, 1.0)
+    # blocks of moments of ordinary size too: zeros and small ones among them decide which way a block goes
+    v[: n // 2] = spread(-60, 20)[: n // 2]
+    m[::1001] = 0.0
+    if eps > 0:
+        v[::997] = 0.0
+    got, want = plain_step(m, v, eps)
+    assert torch.equal(got, want), int((got != want).sum())
+
+
+def test_decayed_moments_of_zero_weights():
+    """Rows of an embedding that get no more gradients: bit for bit, as the moments decay below 2^-100."""
+    params, opt = make([70001], torch.float32, 3, precision="fp32")
+    params[0].data.zero_()
+    opt.step()
+    arena = opt.arenas[0]
+    arena.m.mul_(2.0 ** -85)
+    params[0].data.zero_()
+    params[0].grad.zero_()
+    for step in range(2, 60):
+        params[0].data.zero_()
+        want = restated(*state_of(opt, arena, 0)[:3], params[0].grad.cpu(), step, 0, None, opt)
+        opt.step()
+        assert all(torch.equal(a, b) for a, b in zip(state_of(opt, arena, 0)[:3], want)), step
+
+
 def test_stochastic_rounding_is_unbiased():
     """One value of m and of v repeated n times beside a large one per block: the mean of what is stored is within six
     standard errors of the value; a code's spread is at most half a step (m), half of (q+1)^2 - q^2 steps (v)."""
