@@ -580,7 +580,8 @@ __device__ __forceinline__ void update(const Loaded<I8, W>& in, const Lane<I8, W
         for (int j = 0; j < 4; ++j) {
             p[j] = first_of(p[j], cnt - 2 * j);
             m[j] = first_of(m[j], cnt - 2 * j);
-            root[j] = first_of(root[j], cnt - 2 * j);
+            if constexpr (I8) root[j] = first_of(root[j], cnt - 2 * j);
+            else v[j] = first_of(v[j], cnt - 2 * j);   // not 0 there by itself: 0 times a scale that is not finite
         }
         if (cnt < 4) zeros[0] |= 0x01010101U << (8 * cnt);
         zeros[1] |= cnt <= 4 ? 0x01010101U : cnt < 8 ? 0x01010101U << (8 * (cnt - 4)) : 0U;

@@ -52,7 +52,8 @@ class StateArena:
     ``m``, ``v``: fp32 values, or int8 / uint8 codes with ``m_scale``, ``v_scale`` (one per 256 values; else None);
     ``master``: the fp32 masters of the bf16 parameters, parameter ``i`` at ``master_offsets[i]`` (None for an fp32
     parameter; the buffer is None if the group has no bf16 one); ``steps``: steps taken, int64 per parameter.
-    Values between a parameter's end and the next boundary are zero and stay zero."""
+    Values between a parameter's end and the next boundary are zero and stay zero (but for 8-bit moments whose block has a
+    value that is not finite: the whole block reads back as NaN)."""
 
     def __init__(self, params: list[torch.Tensor], first_index: int, precision: str):
         for p in params:

@@ -240,6 +240,24 @@ def test_padding_stays_zero():
             assert float(rest.abs().max()) == 0.0
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("precision", ["fp32", "int8"])
+@pytest.mark.parametrize("scale", [float("inf"), float("-inf"), float("nan")])
+def test_padding_stays_zero_whatever_the_gradient_scale(precision, dtype, scale):
+    """8-bit moments of such a block are NaN as a whole; the masters' padding and fp32 moments' stays 0."""
+    params, opt = make([3, 300], dtype, 1, precision=precision)
+    opt.step()
+    opt.step(grad_scale=torch.full((1,), scale, device="cuda"))
+    a = opt.arenas[0]
+    planes = [(a.m, a.offsets), (a.v, a.offsets)] if precision == "fp32" else []
+    planes += [(a.master, a.master_offsets)] if a.master is not None else []
+    for flat, offsets in planes:
+        for at, n in zip(offsets, a.numels):
+            rest = flat[at + n:at + -(-n // BLOCK) * BLOCK]
+            assert float(rest.abs().max()) == 0.0
+    assert bool(a.exp_avg_sq()[:3].isnan().all() or a.exp_avg_sq()[:3].isinf().all())
+
+
 def test_small_second_moments_never_become_zero_and_updates_stay_bounded():
     p = torch.nn.Parameter(torch.zeros(512, device="cuda"))
     p.grad = torch.full((512,), 1e-6, device="cuda")
