@@ -250,6 +250,29 @@ def test_special_rows(cols):
     check(far, w, b, 1e-5, False, dy)
 
 
+@pytest.mark.parametrize("cols", [1, 4, 5, 20, 40, 65, 300, 1000, 1023, 4100, 4099, 9001, 12004, 20001, 20004])
+def test_constant_rows_of_large_values(cols):
+    """Every value 2^112, whose sum and mean are exact: h is 0, and dx = r (a - mean a), although -mean r, which h would be
+    beyond the row's end, overflows.  Each of a, its mean (n roundings) and dx rounds: (n + 8) e r (|a| + mean |a|)."""
+    if float(torch.tensor(float(cols)) * (1.0 / torch.tensor(float(cols)))) != 1.0:
+        pytest.skip("the reciprocal's rounding moves the mean")
+    _, w, b, dy = data(40, cols, torch.float32, 13)
+    x = torch.full((40, cols), 2.0 ** 112, device="cuda", requires_grad=True)
+    w.requires_grad_(True)
+    b.requires_grad_(True)
+    eps = 1e-12
+    y = ab.layer_norm(x, w, b, eps=eps)
+    assert torch.equal(y, b.expand(40, cols))
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    a = dy.double() * w.detach().double()
+    r = 1 / math.sqrt(float(torch.tensor(eps)))
+    want = r * (a - a.mean(1, keepdim=True))
+    size = r * (a.abs() + a.abs().mean(1, keepdim=True))
+    assert bool(((dx.double() - want).abs() <= (depth(cols) + 8) * E * size).all())
+    assert float(dw.abs().max()) == 0.0
+    assert bool(((db.double() - dy.double().sum(0)).abs() <= 80 * E * dy.double().abs().sum(0)).all())
+
+
 @pytest.mark.parametrize("rms", [False, True])
 @pytest.mark.parametrize("cols", [5, 40, 300])
 def test_gradients_against_differences(rms, cols):
