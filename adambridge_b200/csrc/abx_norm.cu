@@ -1188,6 +1188,8 @@ int backward_parts(const abx_norm& n, int sms)
     });
 }
 
+constexpr int kMostKept = 220 * 1024;   // bytes of rows that a long kernel keeps in shared memory, at most
+
 // A launch with `bytes` of dynamic shared memory, for this kernel always the same or not; `most` CTAs, or as many as are
 // resident.
 template <auto KERNEL>
@@ -1195,7 +1197,9 @@ int launch_rows(int64_t most, bool all_resident, int threads, size_t bytes, bool
                 const char* what)
 {
     if (bytes > 40960) {   // with the kernels' static shared memory that may exceed what needs no asking
-        const cudaError_t e = cudaFuncSetAttribute((const void*)KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        // always the same for a kernel: a smaller limit would fail a larger row that another thread is about to launch
+        const cudaError_t e = cudaFuncSetAttribute((const void*)KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   same ? (int)bytes : kMostKept);
         if (e != cudaSuccess) return abx::set_error(what, e);
     }
     if (all_resident) {
@@ -1211,8 +1215,8 @@ int launch_rows(int64_t most, bool all_resident, int threads, size_t bytes, bool
 // an SM's 227 KB, one as far as it fits; 0: the row is read again instead.
 int rows_kept(int64_t bytes)
 {
-    constexpr int64_t kHalf = 110 * 1024, kAll = 220 * 1024;
-    return 2 * bytes <= kHalf ? 2 : bytes <= kAll ? 1 : 0;
+    constexpr int64_t kHalf = 110 * 1024;
+    return 2 * bytes <= kHalf ? 2 : bytes <= kMostKept ? 1 : 0;
 }
 
 }  // namespace

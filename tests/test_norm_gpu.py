@@ -322,6 +322,35 @@ def test_another_stream_and_in_place_changes():
         y.sum().backward()
 
 
+def test_long_rows_of_different_lengths_on_two_threads():
+    """The long kernels ask for shared memory by the row's length; calls at the same time do not take each other's away."""
+    import threading
+    lib = native.load()._lib
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    codes: list[set] = [set(), set()]
+    held = []
+    for cols in (27000, 54000):                 # 108 and 216 KB of fp32
+        held.append((torch.ones(1, cols, device="cuda"), torch.empty(1, cols, device="cuda")))
+    torch.cuda.synchronize()
+
+    def work(k):
+        x, y = held[k]
+        spec = native.Norm(x=x.data_ptr(), rows=1, cols=x.shape[1], x_stride=x.shape[1], dtype=native.DT_F32,
+                           w_dtype=native.DT_F32, rms=1, eps=1e-5)
+        for _ in range(5000):
+            codes[k].add(lib.abx_norm_forward(streams[k].cuda_stream, ctypes.byref(spec), y.data_ptr(), None, None))
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert codes == [{0}, {0}]
+    for _, y in held:
+        assert bool(((y - 1 / math.sqrt(1 + 1e-5)).abs() <= 4 * E).all())
+
+
 def test_past_32_bits():
     """More than 2^32 values: the last rows equal the same rows alone."""
     if torch.cuda.get_device_properties(0).total_memory < 80 << 30:
