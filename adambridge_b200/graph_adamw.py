@@ -265,6 +265,18 @@ class GraphAdamW(torch.optim.Optimizer):
         if not group["weight_decay"] >= 0.0:
             raise ValueError(f"invalid weight_decay: {group['weight_decay']}")
 
+    @classmethod
+    def _check_saved_group(cls, group: dict[str, Any], what: str) -> None:
+        for name in ("lr", "betas", "eps", "weight_decay"):
+            if name not in group:
+                raise ValueError(f"{what} has no {name}")
+        cls._check_group(group)
+        for name in ("maximize", "amsgrad"):
+            if group.get(name):
+                raise ValueError(f"{what} has {name}=True, which GraphAdamW does not do")
+        if group["weight_decay"] and not group.get("decoupled_weight_decay", True):
+            raise ValueError(f"{what} adds its weight decay to the gradient; GraphAdamW's is decoupled")
+
     # ------------------------------------------------------------------ the step
 
     def prepare(self) -> "GraphAdamW":
@@ -435,6 +447,8 @@ class GraphAdamW(torch.optim.Optimizer):
             if step < 0:
                 raise ValueError(f"checkpoint parameter {index} has taken {step} steps")
             parsed[index] = (step, master, found)
+        for number, group in enumerate(state_dict["param_groups"]):
+            self._check_saved_group(group, f"checkpoint parameter group {number}")
         rates = [group["lr"] for group in self.param_groups]
         super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
         for group, lr in zip(self.param_groups, rates):

@@ -756,6 +756,28 @@ def test_masters_follow_the_weights_where_a_checkpoint_has_none():
     assert all(torch.equal(p, s) for p, s in zip(params, source))
 
 
+@pytest.mark.parametrize("change, message", [
+    (dict(betas=(1.5, 0.9)), "betas"), (dict(lr=-1.0), "learning rate"), (dict(eps=-1.0), "epsilon"),
+    (dict(weight_decay=float("nan")), "weight_decay"), (dict(maximize=True), "maximize"), (dict(amsgrad=True), "amsgrad"),
+    (dict(lr=torch.zeros(2)), "lr must be"), (dict(decoupled_weight_decay=False), "decoupled"), (dict(eps=None), "no eps")])
+def test_checkpoint_settings_that_it_cannot_follow_are_refused(change, message):
+    """Nothing changes, the learning rate's tensor included."""
+    lr = torch.full((1,), 1e-3, device="cuda")
+    params, opt = make([300], torch.bfloat16, 3, lr=lr)
+    opt.step()
+    saved = opt.state_dict()
+    saved["param_groups"][0].update(change)
+    if "eps" in change and change["eps"] is None:
+        del saved["param_groups"][0]["eps"]
+    before, group = snapshot(params, opt), dict(opt.param_groups[0])
+    with pytest.raises((ValueError, TypeError), match=message):
+        opt.load_state_dict(saved)
+    assert all(torch.equal(a, b) for a, b in zip(before, snapshot(params, opt)))
+    after = opt.param_groups[0]
+    assert after["lr"] is lr and float(lr) == pytest.approx(1e-3)
+    assert all(after[k] == group[k] for k in ("betas", "eps", "weight_decay"))
+
+
 # --------------------------------------------------------------------------- refusals
 
 def test_refusals():
