@@ -228,6 +228,65 @@ def test_stochastic_rounding_is_unbiased():
         assert abs(float(got.mean()) - value) < 6 * step / 2 / math.sqrt(got.numel()) + 1e-5 * value
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("precision, stochastic", [("fp32", True), ("int8", True), ("int8", False)])
+@pytest.mark.parametrize("max_ctas", [1, 3])
+def test_few_ctas_give_the_same_bits(dtype, precision, stochastic, max_ctas):
+    """One CTA that goes through every tile of every tensor, its ring of blocks many times around, writes what many do:
+    weights, moments, scales, masters."""
+    sizes = [70001, 1024, 5, 40960, 1023, 9 * 1024 + 8]
+    kw = dict(precision=precision, stochastic_rounding=stochastic)
+    (one, few), (two, many) = make(sizes, dtype, 3, max_ctas=max_ctas, **kw), make(sizes, dtype, 3, **kw)
+    for step in range(3):
+        for params, opt in ((one, few), (two, many)):
+            new_gradients(params, 30 + step)
+            opt.step(grad_scale=torch.full((1,), 0.7, device="cuda"))
+    assert all(torch.equal(a, b) for a, b in zip(snapshot(one, few), snapshot(two, many)))
+
+
+@pytest.mark.parametrize("codes, stored", [(0.04, 1.0), (0.5, 1.0), (0.999, 1.0), (1.25, None), (7 + 2.0 ** -10, None)])
+def test_stochastic_rounding_near_whole_codes(codes, stored):
+    """What is stored for a root of so many codes.  Below one code it is always one: a positive v never becomes 0.  Above, v's
+    mean is v, within six standard errors and 2^-16 of the gap between the neighbours, as the draw has 16 bits."""
+    n = 256 * 4000
+    p = torch.nn.Parameter(torch.zeros(n, device="cuda"))
+    g = torch.full((n,), codes / 255, device="cuda")
+    g[::256] = 1.0
+    p.grad = g
+    opt = ab.GraphAdamW([p], **HYPER, precision="int8")
+    opt.step()
+    arena = opt.arenas[0]
+    small = torch.arange(n, device="cuda") % 256 != 0
+    q = arena.v[:n][small].double()
+    if stored is not None:
+        assert bool((q == stored).all())
+    else:
+        low = math.floor(codes)
+        gap = 2 * low + 1
+        chance = (codes ** 2 - low ** 2) / gap
+        spread = math.sqrt(chance * (1 - chance) / q.numel())
+        # codes is off by the roundings of g, v, its root and the scale: 6 of 2^-24, relative, twice that in v
+        assert abs(float((q * q).mean()) - codes ** 2) <= gap * (6 * spread + 2.0 ** -16) + 12 * E * codes ** 2
+
+
+@pytest.mark.parametrize("codes", [0.25, 3 + 2.0 ** -10, 100 + 2.0 ** -6])
+def test_stochastic_rounding_of_m_near_whole_codes(codes):
+    """m's mean is m within six standard errors and 2^-16 of a code."""
+    n = 256 * 4000
+    p = torch.nn.Parameter(torch.zeros(n, device="cuda"))
+    g = torch.full((n,), codes / 127, device="cuda")
+    g[::256] = 1.0
+    p.grad = g
+    opt = ab.GraphAdamW([p], **HYPER, precision="int8")
+    opt.step()
+    small = torch.arange(n, device="cuda") % 256 != 0
+    q = opt.arenas[0].m[:n][small].double()
+    part = codes - math.floor(codes)
+    spread = math.sqrt(part * (1 - part) / q.numel())
+    # roundings: g, m, the factor, the product, and of the sum with the draw half of 2^-17 (its step below 128 is 2^-17)
+    assert abs(float(q.mean()) - codes) <= 6 * spread + 2.0 ** -16 + 2.0 ** -18 + 8 * E * codes
+
+
 def test_padding_stays_zero():
     """With eps 0 the padding's update would be 0 / 0."""
     params, opt = make([3, 300], torch.bfloat16, 1, eps=0.0, precision="int8")

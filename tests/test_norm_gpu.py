@@ -110,6 +110,29 @@ def test_many_long_rows(cols, dtype):
     check(x.detach(), w.detach(), None, 1e-5, True, dy, (cols % 16 == 0, True, False))
 
 
+def in_flight(lanes):
+    """Rows that every resident CTA together take at once, at most: 2048 threads per SM."""
+    return torch.cuda.get_device_properties(0).multi_processor_count * 2048 // lanes
+
+
+# vectors of a row, and the least number of threads that own one, forward or backward
+VECTORS = [(8, 8), (16, 8), (32, 16), (64, 32), (128, 32), (256, 128), (512, 256), (768, 256), (1024, 256), (1536, 512),
+           (2048, 512), (2560, 512)]
+SINGLES = [(8, 8), (16, 16), (32, 32), (48, 16), (64, 32), (96, 32), (128, 64), (192, 64), (256, 128), (384, 128), (512, 256),
+           (768, 256), (1024, 512), (1536, 512), (2048, 512), (2560, 512)]
+
+
+@pytest.mark.parametrize("vectors, lanes, aligned", [(*s, True) for s in VECTORS] + [(*s, False) for s in SINGLES])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rms", [False, True])
+def test_several_rows_per_cta(vectors, lanes, aligned, dtype, rms):
+    """Three times the rows that are under way at once and some more: every CTA takes several groups of rows, its ring goes
+    around, its sums are carried from group to group, and the last group has a row for some of its threads only."""
+    cols = vectors * (16 // dtype.itemsize) - (0 if aligned else 1)
+    x, w, b, dy = data(3 * in_flight(lanes) + 13, cols, dtype, cols)
+    check(x, w, None if rms else b, 1e-5, rms, dy)
+
+
 @pytest.mark.parametrize("xt, wt", [(torch.bfloat16, torch.float32), (torch.float32, torch.bfloat16)])
 @pytest.mark.parametrize("cols", [64, 129, 4096, 4100, 20000])
 def test_mixed_types(xt, wt, cols):
