@@ -47,9 +47,12 @@ struct Rows {
     int64_t stride;    // elements between rows
 };
 
+// The memory of a lazily negated view holds the other sign.  (Asked first: resolving goes through torch's dispatcher.)
+Tensor signed_as_read(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 Rows rows_of(const Tensor& given)
 {
-    const Tensor t = given.resolve_neg();   // memory of a lazily negated view holds the other sign
+    const Tensor t = signed_as_read(given);
     const int64_t cols = t.size(-1);
     if (!t.is_contiguous()) {
         const int64_t count = t.numel() / cols;
@@ -97,8 +100,8 @@ abx_norm describe(const Rows& x, const Tensor& weight, const Tensor& bias, doubl
     return n;
 }
 
-Tensor contiguous(const Tensor& t) { return t.defined() ? t.resolve_neg().contiguous() : t; }
-Tensor contiguous(const std::optional<Tensor>& t) { return contiguous(t.value_or(Tensor())); }
+Tensor contiguous(const Tensor& t) { return t.defined() ? signed_as_read(t).contiguous() : t; }
+Tensor contiguous(const std::optional<Tensor>& t) { return t ? contiguous(*t) : Tensor(); }
 
 // y, x as the kernels read it, and where `keep`, the rows' statistics: rstd, then the mean (not for RMS norm)
 std::tuple<Tensor, Tensor, Tensor> forward_norm(const Tensor& x, const std::optional<Tensor>& weight,
@@ -213,12 +216,13 @@ Tensor norm(const Tensor& x, const std::optional<Tensor>& weight, const std::opt
 // The kernel descriptions of one arena's parameters that have a gradient, with the tensors they point at.
 struct Described {
     std::vector<abx_graph_tensor> tensors;
-    std::vector<Tensor> params, keep;
+    std::vector<Tensor> params;   // undefined where there is no gradient
+    std::vector<Tensor> keep;
     c10::Device device{c10::kCUDA, 0};
 };
 
 // `rows`: the arena's descriptions without the addresses of weights and gradients (host, one abx_graph_tensor a row).
-std::unique_ptr<Described> describe_step(const std::vector<Tensor>& params, const Tensor& rows, int64_t device)
+std::unique_ptr<Described> describe_step(std::vector<Tensor> params, const Tensor& rows, int64_t device)
 {
     TORCH_CHECK_VALUE(rows.scalar_type() == at::kLong && rows.is_cpu() && rows.is_contiguous() && rows.dim() == 2
                           && rows.size(0) == (int64_t)params.size() && rows.size(1) * 8 == (int64_t)sizeof(abx_graph_tensor),
@@ -226,13 +230,16 @@ std::unique_ptr<Described> describe_step(const std::vector<Tensor>& params, cons
     auto d = std::make_unique<Described>();
     d->device = c10::Device(c10::kCUDA, (c10::DeviceIndex)device);
     d->tensors.reserve(params.size());
-    d->params.reserve(params.size());
     d->keep.reserve(params.size());
     const auto* row = reinterpret_cast<const abx_graph_tensor*>(rows.const_data_ptr());
-    for (size_t i = 0; i < params.size(); ++i, ++row) {
-        const Tensor& p = params[i];
+    d->params = std::move(params);
+    for (size_t i = 0; i < d->params.size(); ++i, ++row) {
+        Tensor& p = d->params[i];
         Tensor g = p.grad();
-        if (!g.defined()) continue;
+        if (!g.defined()) {
+            p.reset();
+            continue;
+        }
         TORCH_CHECK(p.numel() == row->n && known(p.scalar_type()) && code_of(p.scalar_type()) == row->dtype
                         && p.device() == d->device,
                     "a parameter changed after its state was made (", row->n, " values of dtype code ", row->dtype, " on ",
@@ -245,13 +252,12 @@ std::unique_ptr<Described> describe_step(const std::vector<Tensor>& params, cons
                           g.device(), ", its parameter ", row->n, " on ", d->device);
         if (!g.is_contiguous() || g.is_neg()) {
             const c10::DeviceGuard guard(d->device);
-            g = g.resolve_neg().contiguous();
+            g = signed_as_read(g).contiguous();
         }
         abx_graph_tensor t = *row;
         t.w = p.data_ptr();
         t.g = g.const_data_ptr();
         d->tensors.push_back(t);
-        d->params.push_back(p);
         d->keep.push_back(std::move(g));
     }
     return d;
@@ -269,7 +275,7 @@ void launch_step(const Described& d, uintptr_t shared, const Tensor& ticket, int
                               (int32_t)max_ctas), "abx_graph_adamw");
     // as an operation in place says to autograd: a graph that saved a weight may no longer run backward
     for (const Tensor& p : d.params)
-        if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+        if (p.defined() && !p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
 }
 
 // ---- 8-bit moments -----------------------------------------------------------------------------------
