@@ -13,8 +13,10 @@
 // v = (q s)^2 (q in 0..255, s = max sqrt(v) / 255; the root is the one that the update takes anyway).  A code is
 // the nearest, or one of the two neighbours at random so that the expected value is m or v itself: for v, between
 // (q s)^2 and ((q + 1) s)^2, the upper one with probability (x - q)(x + q) / (2 q + 1), x = sqrt(v) / s.  Without
-// that an average that moves by less than half a code per step would never move.  A positive v never gets code 0,
-// or the next update could divide a moment by eps alone.  A block with a moment that is not finite is stored as NaN.
+// that an average that moves by less than half a code per step would never move.  The draw has 16 bits, so the
+// expected value is off by up to 2^-16 of the gap between the two neighbours.  A positive v never gets code 0, or the
+// next update could divide a moment by eps alone: where its root is below one code it is always stored as one, larger
+// than it is.  A block with a moment that is not finite is stored as NaN.
 //
 // One launch for up to 384 tensors, which streams everything once: 16.1 bytes per parameter with 8-bit moments and
 // bf16 weights.  A warp works the coefficients out again whenever its tensor changes (fp64, from the tensor's step

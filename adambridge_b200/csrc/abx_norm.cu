@@ -8,7 +8,8 @@
 // backward pass reads x and dy once (long rows a second time from shared memory) and writes dx once.  The variance is taken
 // about the mean (a second sum over the registers), so no large squares cancel.  A row is owned by part of a warp, a warp or
 // a CTA, by its length.  HBM bounds rows that start on 16 bytes (layer norm of 32768 x 8192 bf16 values: 174 us forward,
-// 283 backward, 0.94 and 0.87 of the copy bandwidth); instructions those whose values are accessed one by one.
+// 283 backward, 0.94 and 0.87 of the copy bandwidth); instructions those whose values are accessed one by one (8000 x 4097
+// bf16 values: 31 per value forward and 37 backward, against 16 and 19, at the same 0.5 to 0.6 issued per cycle).
 //
 // The weights' gradients are sums over rows: a CTA of the backward kernel goes through many rows and keeps its columns'
 // sums in registers, writes them once to a workspace, and a second small launch adds the CTAs' sums in a fixed order.

@@ -207,8 +207,11 @@ class GraphAdamW(torch.optim.Optimizer):
     r"""AdamW (decoupled weight decay, bias correction) whose whole step is device work on the current stream.
 
     Arguments are AdamBridge's where they have its names.  ``precision`` is ``'int8'`` (8-bit blocks) or ``'fp32'``;
-    ``stochastic_rounding`` rounds 8-bit moments at random, so that their expected values are exact, from a hash of
-    ``seed``, the parameter's index, its step and the element: the same run gives the same bits.  ``lr`` of a group may
+    ``stochastic_rounding`` rounds 8-bit moments at random, so that the expected moment is the moment to within 2^-16 of the
+    gap between its neighbouring codes, by a hash of ``seed``, the parameter's index, its step and the element: the same run
+    gives the same bits.  A second moment whose root is below one code of its block (1/255 of the block's largest) is the
+    exception, with either rounding: it is stored as one code, so that it never reads as zero, and such an element moves less
+    than its own moment would have it.  ``lr`` of a group may
     be a one-element float32 or float64 CUDA tensor, read by every replay of a captured step; a float is captured as
     it is.  ``max_ctas`` caps the CTAs of a launch (0: all).
 
@@ -298,7 +301,7 @@ class GraphAdamW(torch.optim.Optimizer):
         ``grad_scale`` and ``found_inf`` are one-element float32 CUDA tensors: every gradient is multiplied by the
         first inside the kernel, and where the second is not zero the step changes nothing, step counts included.
         After :meth:`clip_grad_norm_` the clip coefficient is the scale, and a step whose gradient norm is not finite
-        changes nothing either."""
+        changes nothing either.  For autograd the step is a change in place of the parameters that it describes."""
         loss = None
         if closure is not None:
             with torch.enable_grad():

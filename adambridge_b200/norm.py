@@ -23,7 +23,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
 
     ``x`` is float32 or bfloat16, of any shape and strides (rows that are not evenly spaced, or not contiguous, are
     copied first); ``weight`` and ``bias``, each optional, are float32 or bfloat16 vectors of one dtype, which need not be
-    ``x``'s.  All arithmetic is fp32; ``y`` and the gradients are rounded once to ``x``'s and the weight's dtype.  Runs on
+    ``x``'s.  All arithmetic is fp32, so a row whose sum, or whose sum of squared deviations, passes the range of fp32 gives
+    what elementary fp32 operations give (NaN, or a deviation of infinity); ``y`` and the gradients are rounded once to ``x``'s and the weight's dtype.  Runs on
     the current stream of ``x``'s device.  Gradients are those of first order and reverse mode: differentiating
     them raises, and so do forward-mode tangents and traces (``torch.jit.trace``, ``make_fx``, fake tensors)."""
     return native.torch_ops().norm(x, weight, bias, eps, False)

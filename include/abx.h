@@ -310,7 +310,7 @@ typedef struct abx_graph_step {
     const float* norm;      /* not finite: nothing changes */
     int32_t lr_f64;
     int32_t moments;        /* ABX_DT_F32 or ABX_DT_I8 */
-    int32_t stochastic;     /* ABX_DT_I8: round the codes at random (unbiased) instead of to the nearest */
+    int32_t stochastic;     /* ABX_DT_I8: round the codes at random, to keep expected values, instead of to the nearest */
     uint32_t seed;
 } abx_graph_step;
 
