@@ -650,6 +650,24 @@ def test_a_clip_on_one_stream_and_its_step_on_another(dtype):
     del taken
 
 
+def test_a_captured_clip_on_a_forked_stream():
+    """Both in one capture, the clip on a stream that the capture forks and joins."""
+    (params, opt), (want, plain) = (make([300, 5000], torch.bfloat16, 6) for _ in range(2))
+    opt.prepare()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            opt.clip_grad_norm_(1e-3)
+        torch.cuda.current_stream().wait_stream(side)
+        opt.step()
+    for _ in range(3):
+        graph.replay()
+        plain.clip_grad_norm_(1e-3)
+        plain.step()
+    assert all(torch.equal(a, b) for a, b in zip(snapshot(params, opt), snapshot(want, plain)))
+
+
 def test_a_clip_without_gradients_takes_the_last_one_back():
     params, opt = make([300], torch.float32, 6, precision="fp32")
     other, plain = make([300], torch.float32, 6, precision="fp32")
