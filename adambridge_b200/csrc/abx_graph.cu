@@ -929,7 +929,7 @@ int run_batch(const abx_graph_tensor* t, const int32_t* order, int32_t count, co
     const float high = (float)((1.0 - h.beta2) * 0x1p48), low = kLeastPlain;
     std::memcpy(&a.plain_low, &low, 4);
     std::memcpy(&a.plain_high, &high, 4);
-    if (a.eps > 0x1p24f) a.plain_high = 0;
+    if (!(a.eps >= 0.0f && a.eps <= 0x1p24f)) a.plain_high = 0;
     a.zero_is_plain = a.eps >= 0x1p-60f;
     int64_t next = 0;
     for (int32_t j = 0; j < count; ++j) {
